@@ -2,8 +2,8 @@
 
 ``RoPE(positions)`` returns half-dim ``(cos, sin)`` of shape ``[..., S, 1, D/2]``
 (fp32 unless ``dtype`` is set); ``RoPE.rotate`` applies the half-split (HF) or
-interleaved rotation in fp32 and rounds once. On CUDA the half-split case is one
-fused kernel (``priml_b200.ops.rotary``) reading q, k and the table once.
+interleaved rotation in fp32 and rounds once. On CUDA this is a kernel
+(``priml_b200.ops.rotary``) reading q, k and the table once.
 
 Inverse frequencies are rebuilt on every device move: ``base ** x`` differs in
 the last bit between host and device math libraries, so a device-built table is
@@ -127,8 +127,8 @@ class RoPE(nn.Module):
             sin = torch.cat([sin, torch.zeros(pad, dtype=sin.dtype, device=sin.device)], dim=seq_dim)
         rot = cos.shape[-1] * 2
         d = q.shape[-1]
-        if not interleave and rot == d and q.ndim == 4 and cos.ndim == 3 and cos.shape[-2] == 1:
-            return ops.rotary(q, k, cos, sin)
+        if q.ndim == 4 and ((not interleave and rot == d and cos.ndim == 3 and cos.shape[-2] == 1) or ops.use_native(q)):
+            return ops.rotary(q, k, cos, sin, interleave=interleave)
         if rot < d:
             qr, qp = q[..., :rot], q[..., rot:]
             kr, kp = k[..., :rot], k[..., rot:]

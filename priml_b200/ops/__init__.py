@@ -19,9 +19,11 @@ from priml_b200.ops import reference
 from priml_b200.ops._loader import native, native_available
 
 __all__ = [
+    "CACHE_BLOCK",
     "adamw_",
     "add_rms_norm",
     "attention",
+    "cache_attention",
     "cross_entropy",
     "decode_attention",
     "grouped_swiglu_experts",
@@ -36,6 +38,7 @@ __all__ = [
     "reference_forced",
     "rms_norm",
     "rotary",
+    "rotary_append",
     "swiglu",
     "swiglu_mlp",
     "use_native",
@@ -96,13 +99,26 @@ def add_rms_norm(x: Tensor, d: Tensor | None, weight: Tensor | None, eps: float 
     return h, reference.rms_norm(h, weight, eps)
 
 
-def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> tuple[Tensor, Tensor]:
-    """Half-split RoPE of ``[B, S, H, D]`` q/k with ``[S, 1, D/2]`` fp32 factors."""
-    if use_native(q) and q.dtype == torch.bfloat16 and cos.shape[-1] * 2 == q.shape[-1]:
+def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, interleave: bool = False) -> tuple[Tensor, Tensor]:
+    """RoPE of ``[B, S, H, D]`` q and ``[B, S, Hk, D]`` k by fp32 half-width factors.
+
+    ``cos`` and ``sin`` are ``[S, 1, R/2]`` (one table), ``[B, S, 1, R/2]`` (positions per sequence) or
+    have a head axis of their own; the first ``R`` channels of a head are rotated, the others copied.
+    The pairs are channels ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleave``. The rotation is
+    computed in fp32 and rounded once. On CUDA q and k take one kernel (bf16, fp16, fp32), and its
+    transpose in the backward; factors that need a gradient take the torch operations.
+    """
+    if use_native(q) and not interleave and q.dtype == torch.bfloat16 and cos.ndim == 3 and cos.shape[-1] * 2 == q.shape[-1]:
+        if cos.shape[-2] == 1:
+            from priml_b200.ops import functional
+
+            return functional.rotary(q, k, cos, sin)
+    if use_native(q):
         from priml_b200.ops import functional
 
-        return functional.rotary(q, k, cos, sin)
-    return reference.rotate_half(q, cos, sin), reference.rotate_half(k, cos, sin)
+        if functional.rotary_any_supported(q, k, cos, sin):
+            return functional.rotary_any(q, k, cos, sin, interleave)
+    return reference.rotate(q, cos, sin, interleave), reference.rotate(k, cos, sin, interleave)
 
 
 def attention(
@@ -213,6 +229,121 @@ def decode_attention(
             -1 if window is None else int(window),
         )  # fmt: skip
     return reference.decode_attention(q, k_cache, v_cache, lengths, scale=float(scale), window=window)
+
+
+CACHE_BLOCK = reference.CACHE_BLOCK
+
+
+def _check_cache(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor, lengths: Tensor) -> None:
+    """Refuse caches that do not belong together, on any device."""
+    b, d = q.shape[0], q.shape[-1]
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[0] != b or k_cache.shape[-1] != d:
+        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} do not fit queries {tuple(q.shape)}.")
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"an 8-bit cache holds float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}.")
+    want = (*k_cache.shape[:2], -(-k_cache.shape[2] // CACHE_BLOCK))
+    for name, f in (("k", k_scale), ("v", v_scale)):
+        if tuple(f.shape) != want or f.dtype != torch.float32:
+            raise ValueError(f"{name} scales must be fp32 {want}, got {f.dtype} {tuple(f.shape)}.")
+    if tuple(lengths.shape) != (b,) or lengths.is_floating_point():
+        raise ValueError(f"lengths must be {b} integers, got {lengths.dtype} {tuple(lengths.shape)}.")
+    if any(x.device != q.device for x in (k_cache, v_cache, k_scale, v_scale, lengths)):
+        raise ValueError("the caches, their scales and the lengths must be on the queries' device.")
+
+
+def rotary_append(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    k_cache: Tensor,
+    v_cache: Tensor,
+    k_scale: Tensor,
+    v_scale: Tensor,
+    lengths: Tensor,
+    *,
+    cos: Tensor | None = None,
+    sin: Tensor | None = None,
+    interleave: bool = False,
+) -> Tensor:
+    """Rotate ``s`` new tokens per sequence and append their keys and values to 8-bit caches, in place.
+
+    ``q`` is ``[B, s, H, D]``, ``k`` and ``v`` ``[B, s, Hkv, D]``; token ``i`` of sequence ``b`` takes
+    cache row and position ``lengths[b] + i`` (int32, on the device; not changed here). ``cos`` and
+    ``sin`` are tables ``[positions, R/2]`` that are read at those positions (the last row past their
+    end); q and k are rotated as :func:`rotary` does it. Without them nothing is rotated.
+
+    The caches are ``float8_e4m3fn`` ``[B, Hkv, T, D]``; ``k_scale`` / ``v_scale`` (fp32
+    ``[B, Hkv, ceil(T / 32)]``) hold one power of two per 32 rows and head, the least one with which the
+    rows stay within e4m3's range: a row stands for ``row * scale``. Appending to a block that holds rows
+    already keeps its scale or, for larger values, raises it and requantises those rows. Values that are
+    not finite are stored as NaN. Tokens past ``T`` are not stored. Returns the rotated q.
+
+    On CUDA with bf16 and 64 or 128 channels a head this is one kernel (``csrc/rotary.cu``).
+    """
+    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together.")
+    if k.shape[2] != k_cache.shape[1]:
+        raise ValueError(f"{k.shape[2]} key heads for a cache of {k_cache.shape[1]}.")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together.")
+    if cos is not None and (cos.ndim != 2 or cos.shape != sin.shape or not 2 <= 2 * cos.shape[1] <= q.shape[-1] or cos.shape[0] < 1):
+        raise ValueError(f"cos and sin must be [positions, R/2] tables with 2 <= R <= {q.shape[-1]}, got {tuple(cos.shape)}.")
+    _check_cache(q, k_cache, v_cache, k_scale, v_scale, lengths)
+    if any(x.requires_grad for x in (q, k, v)) and torch.is_grad_enabled():
+        raise RuntimeError("rotary_append has no gradient: call it under torch.no_grad().")
+    if use_native(q) and q.shape[-1] in (64, 128) and all(x.dtype == torch.bfloat16 for x in (q, k, v)):
+        return native().rotary_append(
+            q, k, v, k_cache, v_cache, k_scale, v_scale, lengths.to(torch.int32).contiguous(), cos, sin, interleave
+        )
+    return reference.rotary_append(q, k, v, k_cache, v_cache, k_scale, v_scale, lengths, cos, sin, interleave)
+
+
+def cache_attention(
+    q: Tensor,
+    k_cache: Tensor,
+    v_cache: Tensor,
+    k_scale: Tensor,
+    v_scale: Tensor,
+    lengths: Tensor,
+    *,
+    scale: float | None = None,
+    window: int | None = None,
+    offset: int = 0,
+) -> Tensor:
+    """Attention of each sequence's last tokens over its 8-bit cache (see :func:`rotary_append`).
+
+    ``q`` is ``[B, H, D]`` (one token per sequence) or ``[B, s, H, D]`` (a chunk). ``lengths[b] + offset``
+    rows of sequence ``b`` are filled, the chunk's own included: query ``i`` stands at position
+    ``lengths[b] + offset - s + i`` and sees the rows up to its own, with ``window`` only those not more
+    than ``window`` behind it. A query that sees no row gives zeros; rows that a query does not see may
+    hold anything. Query head ``h`` reads KV head ``h // (H / Hkv)``. The lengths stay on the device, so
+    the call can be captured in a CUDA graph. Returns ``q``'s shape.
+
+    On CUDA with bf16 queries and 64 or 128 channels a head this runs ``csrc/cache_attention*.cu``.
+    """
+    if q.ndim not in (3, 4):
+        raise ValueError(f"q must be [B, H, D] or [B, s, H, D], got {tuple(q.shape)}.")
+    q4 = q[:, None] if q.ndim == 3 else q
+    _check_cache(q4, k_cache, v_cache, k_scale, v_scale, lengths)
+    if k_cache.shape[1] < 1 or q4.shape[2] % k_cache.shape[1]:
+        raise ValueError(f"{q4.shape[2]} query heads are not a multiple of {k_cache.shape[1]} KV heads.")
+    if window is not None and window < 0:
+        window = None
+    if not 0 <= offset < 1 << 31:
+        raise ValueError(f"offset must be a token count, got {offset}.")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("cache_attention has no gradient: call it under torch.no_grad().")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if use_native(q) and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
+        out = native().cache_attn(
+            q4, k_cache, v_cache, k_scale, v_scale, lengths.to(torch.int32).contiguous(), offset, scale,
+            -1 if window is None else int(window),
+        )  # fmt: skip
+    else:
+        out = reference.cache_attention(
+            q4, k_cache, v_cache, k_scale, v_scale, lengths, scale=scale, window=window, offset=offset
+        )
+    return out[:, 0] if q.ndim == 3 else out
 
 
 def cross_entropy(logits: Tensor, targets: Tensor, *, ignore_index: int = -100, softcap: float | None = None) -> Tensor:

@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstring>
 #include <memory>
 #include <mutex>
@@ -705,6 +706,212 @@ Tensor decode_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.status = status_ptr();
   pb::decode_attn(p, B, D, stream());
+  return out;
+}
+
+// Rotary embedding of q [B, S, H, D] and k [B, S, Hk, D] (bf16, fp16 or fp32; contiguous channels, any
+// other strides): the first 2 * cos.size(-1) channels, half-split or interleaved pairs. cos / sin: fp32
+// [S, Hf, R/2] or [B, S, Hf, R/2] with batch and head axes of size 1 where shared.
+std::vector<Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, bool interleave,
+                           double sign) {
+  check_cuda(q, "q");
+  check_cuda(k, "k");
+  PB_CHECK(k.device() == q.device(), "q and k must be on one device");
+  PB_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
+           "q and k must be [B, S, heads, D] of one batch, length and head dim");
+  PB_CHECK(q.scalar_type() == k.scalar_type(), "q and k must share a dtype");
+  const auto st = q.scalar_type();
+  PB_CHECK(st == torch::kBFloat16 || st == torch::kFloat32 || st == torch::kFloat16, "q must be bf16, fp16 or fp32");
+  const int64_t B = q.size(0), S = q.size(1), H = q.size(2), Hk = k.size(2), D = q.size(3);
+  PB_CHECK(q.stride(3) == 1 && k.stride(3) == 1, "channels must be contiguous");
+  PB_CHECK(cos.sizes() == sin.sizes() && (cos.dim() == 3 || cos.dim() == 4), "cos and sin must be [(B,) S, heads, R/2]");
+  auto c = aux(cos, q, torch::kFloat32);
+  auto s = aux(sin, q, torch::kFloat32);
+  const int64_t half = c.size(-1), Hf = c.size(-2);
+  PB_CHECK(half >= 1 && 2 * half <= D, "the rotated channels must fit the head dim");
+  PB_CHECK(c.size(-3) == S && (c.dim() == 3 || c.size(0) == 1 || c.size(0) == B), "cos must hold one row per token");
+  PB_CHECK(Hf == 1 || (Hf == H && Hf == Hk), "cos must be shared by the heads or hold one row per head");
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto qo = torch::empty({B, S, H, D}, q.options());
+  auto ko = torch::empty({B, S, Hk, D}, k.options());
+  if (B * S * D == 0 || H + Hk == 0) return {qo, ko};
+  PB_CHECK(B * S < (1LL << 31) && (H + Hk) * D < (1LL << 22), "sizes out of range");
+  pb::RotaryParams p{};
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+  p.k_sb = k.stride(0), p.k_ss = k.stride(1), p.k_sh = k.stride(2);
+  p.q_out = qo.data_ptr();
+  p.k_out = ko.data_ptr();
+  p.cos = c.data_ptr<float>();
+  p.sin = s.data_ptr<float>();
+  p.f_sh = Hf == 1 ? 0 : half;
+  p.f_ss = Hf * half;
+  p.f_sb = c.dim() == 4 && c.size(0) == B ? S * Hf * half : 0;
+  p.tokens = B * S;
+  p.S = static_cast<int>(S), p.H = static_cast<int>(H), p.Hk = static_cast<int>(Hk);
+  p.D = static_cast<int>(D), p.R = static_cast<int>(2 * half);
+  p.sign = static_cast<float>(sign);
+  p.interleave = interleave;
+  pb::rotary(p, st == torch::kBFloat16 ? 0 : (st == torch::kFloat32 ? 1 : 2), stream());
+  return {qo, ko};
+}
+
+// The checks that the append and the attention share: an e4m3 cache [B, Hkv, T, D] with contiguous,
+// 16-byte aligned rows, and its fp32 scales [B, Hkv, ceil(T / 32)].
+void check_cache(const Tensor& cache, const Tensor& scale, const Tensor& ref, int64_t B, int64_t Hkv, int64_t T,
+                 int64_t D, const char* name) {
+  const std::string n(name);
+  PB_CHECK(cache.is_cuda() && cache.scalar_type() == torch::kFloat8_e4m3fn && cache.device() == ref.device(),
+           n + " cache must be float8_e4m3fn on the query's device");
+  PB_CHECK(cache.dim() == 4 && cache.size(0) == B && cache.size(1) == Hkv && cache.size(2) == T && cache.size(3) == D,
+           n + " cache must be [B, Hkv, T, D]");
+  PB_CHECK(cache.stride(3) == 1 && (cache.stride(2) == D || T <= 1), n + " cache rows must be contiguous");
+  PB_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0 && cache.stride(0) % 16 == 0 &&
+               cache.stride(1) % 16 == 0,
+           n + " cache base and strides must be 16-byte aligned");
+  PB_CHECK(scale.is_cuda() && scale.scalar_type() == torch::kFloat32 && scale.device() == ref.device() &&
+               scale.dim() == 3 && scale.size(0) == B && scale.size(1) == Hkv &&
+               scale.size(2) == (T + pb::kCacheBlock - 1) / pb::kCacheBlock && (scale.stride(2) == 1 || scale.size(2) <= 1),
+           n + " scales must be fp32 [B, Hkv, ceil(T / 32)] with contiguous blocks");
+}
+
+void check_lengths(const Tensor& lengths, const Tensor& ref, int64_t B) {
+  PB_CHECK(lengths.is_cuda() && lengths.device() == ref.device() && lengths.scalar_type() == torch::kInt32 &&
+               lengths.dim() == 1 && lengths.numel() == B && (lengths.stride(0) == 1 || B <= 1),
+           "lengths must be contiguous int32 [B] on the query's device");
+}
+
+// A tensor the append writes must not map two of its (sequence, head) planes onto the same memory.
+void check_planes(const Tensor& t, const char* name) {
+  const int64_t plane = t.dim() == 4 ? t.size(2) * t.size(3) : t.size(2);
+  const int64_t b = t.size(0), h = t.size(1);
+  const int64_t sb = t.stride(0), sh = t.stride(1);
+  const bool heads_in = h <= 1 || sh >= plane, seqs_in = b <= 1 || sb >= plane;
+  const int64_t heads_span = h <= 1 ? plane : (h - 1) * sh + plane, seqs_span = b <= 1 ? plane : (b - 1) * sb + plane;
+  PB_CHECK(t.numel() == 0 || (heads_in && seqs_in && (b <= 1 || h <= 1 || sb >= heads_span || sh >= seqs_span)),
+           std::string(name) + " must not overlap itself");
+}
+
+// Channels contiguous and rows 16-byte aligned, as the vector loads need them.
+Tensor rows16(const Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && (t.stride(d) % 8 == 0 || t.size(d) <= 1);
+  return ok ? t : t.contiguous();
+}
+
+// Rotates q and k [B, s, H | Hkv, D] at positions lengths[b] + i (cos / sin: fp32 [P, R/2], or none) and
+// appends k and v to the 8-bit caches at those rows; returns the rotated q (q itself without factors).
+Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tensor& k_cache, Tensor& v_cache,
+                     Tensor& k_scale, Tensor& v_scale, const Tensor& lengths, const c10::optional<Tensor>& cos,
+                     const c10::optional<Tensor>& sin, bool interleave) {
+  for (const Tensor* t : {&q_, &k_, &v_})
+    PB_CHECK(t->is_cuda() && t->scalar_type() == torch::kBFloat16 && t->dim() == 4 && t->device() == q_.device(),
+             "q, k and v must be bf16 [B, s, heads, D] on one device");
+  const int64_t B = q_.size(0), s = q_.size(1), H = q_.size(2), D = q_.size(3), Hkv = k_.size(2);
+  PB_CHECK(D == 64 || D == 128, "the 8-bit cache covers head dims 64 and 128");
+  PB_CHECK(k_.sizes() == v_.sizes() && k_.size(0) == B && k_.size(1) == s && k_.size(3) == D,
+           "k and v must be [B, s, Hkv, D] beside q");
+  PB_CHECK(k_cache.dim() == 4, "k cache must be [B, Hkv, T, D]");
+  const int64_t T = k_cache.size(2);
+  check_cache(k_cache, k_scale, q_, B, Hkv, T, D, "k");
+  check_cache(v_cache, v_scale, q_, B, Hkv, T, D, "v");
+  check_lengths(lengths, q_, B);
+  check_planes(k_cache, "k cache");
+  check_planes(v_cache, "v cache");
+  check_planes(k_scale, "k scales");
+  check_planes(v_scale, "v scales");
+  PB_CHECK(cos.has_value() == sin.has_value(), "cos and sin come together");
+  PB_CHECK(T < (1LL << 31) - 64 && B * s < (1LL << 30) && B * Hkv * (s / pb::kCacheBlock + 2) < (1LL << 29),
+           "sizes out of range");
+  const c10::cuda::CUDAGuard guard(q_.device());
+  auto q = rows16(q_), k = rows16(k_), v = rows16(v_);
+  pb::AppendParams p{};
+  Tensor c, n, out = q_;
+  if (cos.has_value()) {
+    PB_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes() && cos->size(0) >= 1 && cos->size(1) >= 1 &&
+                 2 * cos->size(1) <= D,
+             "cos and sin must be [positions, R/2] tables with R <= D");
+    c = aux(*cos, q_, torch::kFloat32);
+    n = aux(*sin, q_, torch::kFloat32);
+    out = torch::empty({B, s, H, D}, q_.options());
+    p.cos = c.data_ptr<float>();
+    p.sin = n.data_ptr<float>();
+    p.table_rows = c.size(0);
+    p.R = static_cast<int>(2 * c.size(1));
+    p.q_out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  }
+  if (B * s == 0) return out;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  p.k = reinterpret_cast<const __nv_bfloat16*>(k.data_ptr());
+  p.v = reinterpret_cast<const __nv_bfloat16*>(v.data_ptr());
+  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+  p.k_sb = k.stride(0), p.k_ss = k.stride(1), p.k_sh = k.stride(2);
+  p.v_sb = v.stride(0), p.v_ss = v.stride(1), p.v_sh = v.stride(2);
+  p.k_cache = static_cast<uint8_t*>(k_cache.data_ptr());
+  p.v_cache = static_cast<uint8_t*>(v_cache.data_ptr());
+  p.kc_sb = k_cache.stride(0), p.kc_sh = k_cache.stride(1);
+  p.vc_sb = v_cache.stride(0), p.vc_sh = v_cache.stride(1);
+  p.k_scale = k_scale.data_ptr<float>();
+  p.v_scale = v_scale.data_ptr<float>();
+  p.ks_sb = k_scale.stride(0), p.ks_sh = k_scale.stride(1);
+  p.vs_sb = v_scale.stride(0), p.vs_sh = v_scale.stride(1);
+  p.lengths = lengths.data_ptr<int>();
+  p.B = static_cast<int>(B), p.s = static_cast<int>(s), p.H = static_cast<int>(H), p.Hkv = static_cast<int>(Hkv);
+  p.T = static_cast<int>(T);
+  pb::rotary_append(p, static_cast<int>(D), interleave, stream());
+  return out;
+}
+
+// q [B, s, H, D] over 8-bit caches; query i of sequence b stands at position n - s + i with
+// n = min(lengths[b] + offset, T). Returns [B, s, H, D] (contiguous bf16).
+Tensor cache_attn(const Tensor& q_, const Tensor& k, const Tensor& v, const Tensor& k_scale, const Tensor& v_scale,
+                  const Tensor& lengths, int64_t offset, double scale, int64_t window) {
+  PB_CHECK(q_.is_cuda() && q_.scalar_type() == torch::kBFloat16 && q_.dim() == 4, "q must be CUDA bf16 [B, s, H, D]");
+  const int64_t B = q_.size(0), s = q_.size(1), H = q_.size(2), D = q_.size(3);
+  PB_CHECK(D == 64 || D == 128, "the 8-bit cache covers head dims 64 and 128");
+  PB_CHECK(k.dim() == 4, "k cache must be [B, Hkv, T, D]");
+  const int64_t Hkv = k.size(1), T = k.size(2);
+  check_cache(k, k_scale, q_, B, Hkv, T, D, "k");
+  check_cache(v, v_scale, q_, B, Hkv, T, D, "v");
+  check_lengths(lengths, q_, B);
+  PB_CHECK(Hkv > 0 && H % Hkv == 0, "query heads must be a multiple of the KV heads");
+  PB_CHECK(T < (1LL << 31) - 64 && s * (H / Hkv) < (1LL << 30) && B * s * H < (1LL << 31), "sizes out of range");
+  PB_CHECK(offset >= 0 && offset < (1LL << 31), "offset must be a token count");
+  const c10::cuda::CUDAGuard guard(q_.device());
+  auto q = rows16(q_);
+  auto out = torch::empty({B, s, H, D}, q.options());
+  if (out.numel() == 0) return out;
+  if (T == 0) return out.zero_();
+  const int64_t step = pb::cache_attn_max_seqs();
+  for (int64_t b0 = 0; b0 < B; b0 += step) {
+    const int64_t nb = std::min(step, B - b0);
+    pb::CacheAttnParams p{};
+    p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()) + b0 * q.stride(0);
+    p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+    p.k = static_cast<const uint8_t*>(k.data_ptr()) + b0 * k.stride(0);
+    p.v = static_cast<const uint8_t*>(v.data_ptr()) + b0 * v.stride(0);
+    p.k_sb = k.stride(0), p.k_sh = k.stride(1), p.v_sb = v.stride(0), p.v_sh = v.stride(1);
+    p.k_scale = k_scale.data_ptr<float>() + b0 * k_scale.stride(0);
+    p.v_scale = v_scale.data_ptr<float>() + b0 * v_scale.stride(0);
+    p.ks_sb = k_scale.stride(0), p.ks_sh = k_scale.stride(1);
+    p.vs_sb = v_scale.stride(0), p.vs_sh = v_scale.stride(1);
+    p.lengths = lengths.data_ptr<int>() + b0;
+    p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()) + b0 * s * H * D;
+    p.B = static_cast<int>(nb), p.s = static_cast<int>(s), p.H = static_cast<int>(H), p.Hkv = static_cast<int>(Hkv);
+    p.T = static_cast<int>(T), p.group = static_cast<int>(H / Hkv);
+    p.offset = static_cast<int>(offset);
+    p.window = static_cast<int>(std::min<int64_t>(window, T));
+    p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+    p.status = status_ptr();
+    long long part_floats = 0, plan_words = 0;
+    pb::cache_attn_plan(p, static_cast<int>(D), &part_floats, &plan_words);
+    auto part = torch::empty({part_floats}, q.options().dtype(torch::kFloat32));
+    auto plan = torch::empty({plan_words}, q.options().dtype(torch::kInt64));
+    p.part = part.data_ptr<float>();
+    p.plan = reinterpret_cast<long long*>(plan.data_ptr<int64_t>());
+    pb::cache_attn(p, static_cast<int>(D), stream());
+  }
   return out;
 }
 
@@ -1472,6 +1679,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q"), py::arg("c_kv"), py::arg("k_pe"), py::arg("lengths"), py::arg("scale"));
   m.def("decode_attn", &decode_attn, "one-token decode attention over a KV cache with device lengths",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("lengths"), py::arg("scale"), py::arg("window") = -1);
+  m.def("rotary", &rotary, "rotary embedding of q and k in any layout", py::arg("q"), py::arg("k"), py::arg("cos"),
+        py::arg("sin"), py::arg("interleave"), py::arg("sign"));
+  m.def("rotary_append", &rotary_append, "rotary embedding fused with the append to an 8-bit cache", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("lengths"), py::arg("cos"), py::arg("sin"), py::arg("interleave"));
+  m.def("cache_attn", &cache_attn, "attention over an 8-bit KV cache with device lengths", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("k_scale"), py::arg("v_scale"), py::arg("lengths"), py::arg("offset"), py::arg("scale"),
+        py::arg("window"));
   m.def("attn_fwd", &attn_fwd, "flash attention forward (tcgen05); trace: optional int32 [8 * CTAs] progress record",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("causal"), py::arg("window"),
         py::arg("trace") = py::none());

@@ -1,0 +1,632 @@
+// Attention of a few query rows per KV head over an 8-bit cache (one-token decode above all).
+//
+//   o_r = sum_t softmax_t(scale q_r . K_t) V_t,   K_t = 2^ek k_t,  V_t = 2^ev v_t
+//
+// with e4m3 rows k_t, v_t and one scale per 32 cache rows and head. A row r is one (token, query
+// head of the KV head's group); it sees the keys at or before its token's position.
+//
+// Bound: 2 D + 1/4 bytes per visible key and KV head, read once, against group x 4 D flops: HBM.
+// Per SM that is about 23 cached values per clock, each needing `group` multiply-adds and a
+// conversion, which the fp32 pipes cannot do at group 4 and up. So the products run on the
+// tensor cores as m16n8k16 f16 products with keys (then channels) on M and query rows on N: the
+// e4m3 operand converts exactly to f16 in registers, straight from 16-byte global loads, with no
+// shared memory in between. tcgen05 would need the converted tile in shared memory and 128 rows
+// of M per product; here N = 8 rows are useful and the pipes idle anyway.
+//
+//   S^T = K Q^T    A: K rows (lane g holds rows g, g + 8), B: Q.  The contraction index d is
+//                  permuted so that a lane's 16 consecutive bytes of a row are four k-steps.
+//   O^T = V^T P^T  A: V^T.  A lane holds 16 (D = 64: 8) consecutive channels of 4 keys; bytes of
+//                  neighbouring keys are interleaved (prmt) into the k-pairs of the fragment.
+//                  B: P^T from S^T by an 8 x 8 transpose (movmatrix).
+// One scale belongs to one 32-key step, so K's scale multiplies the scores and V's the step's own
+// accumulator, which is then added to the running one (the same multiply-add carries the
+// softmax's rescaling). Query rows are normalised by a power of two to fit f16 (exact; the factor
+// goes to the scores). P is rounded to f16 as 2^10 p: half a step is 2^-11 relative down to
+// p = 2^-24, less than bf16's 2^-9 of the output, and far tails stay above zero.
+//
+// Work split: the key blocks of all (sequence, KV head, row group) items form one list, cut into
+// equal runs over the grid on the device from the lengths, so ragged batches load all SMs alike
+// and nothing depends on the host knowing a length. A run's piece of an item is written as an
+// unnormalised partial (slot = CTA + item: both only grow along the list, so slots are unique);
+// an item inside one run is finished at once. A second kernel merges the partials in slot order.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace pb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kMaxSeqs = 1024;  // sequences per launch (prefix table in shared memory)
+constexpr int kMinRun = 4;      // key blocks per CTA at least: one per warp
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two e4m3 bytes -> two halves (exact).
+__device__ __forceinline__ uint32_t f16x2_of(uint32_t two_bytes) {
+  uint32_t d;
+  asm("{\n.reg .b16 h;\ncvt.u16.u32 h, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(d) : "r"(two_bytes));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Streaming 16-byte load (each cached byte is used once).
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// Bytes that hold an e4m3 NaN (0x7f, 0xff) as 0xff, others 0.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  const uint32_t m = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return (m >> 7) * 255u;
+}
+
+struct Item {
+  long long b;
+  int hk, rg;        // KV head, row group
+  long long n;       // keys in the cache, at most T
+  int first_block;   // first key block that any row of the sequence sees
+  int blocks;
+};
+
+// Keys of sequence b (0 .. T) and its visible key blocks.
+__device__ __forceinline__ int seq_blocks(const CacheAttnParams& p, int b, long long& n, int& first) {
+  n = static_cast<long long>(p.lengths[b]) + p.offset;
+  n = n < 0 ? 0 : (n > p.T ? p.T : n);
+  long long lo = 0;
+  if (p.window >= 0) {
+    lo = n - p.s - p.window;
+    lo = lo < 0 ? 0 : lo;
+  }
+  first = static_cast<int>(lo / kCacheBlock);
+  return static_cast<int>((n + kCacheBlock - 1) / kCacheBlock) - first;
+}
+
+template <int D, int RT>
+struct Step {  // one warp's raw bytes of a 32-key step
+  static constexpr int KV = D / 64;  // 16-byte K pieces per row half... (16 bytes at hf * 64 + t * 16)
+  uint4 k[4][KV];                    // rows g, g + 8, g + 16, g + 24
+  uint32_t v[8][D / 32];             // keys 2t, 2t+1, 2t+8, 2t+9 (+16); D / 8 bytes at g * D / 8
+  float ks, vs;
+};
+
+template <int D, int RT>
+__device__ __forceinline__ void load_k(Step<D, RT>& st, const uint8_t* k, int base, int n, int g, int t) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = base + i * 8 + g;
+#pragma unroll
+    for (int hf = 0; hf < D / 64; ++hf)
+      st.k[i][hf] = row < n ? load16(k + static_cast<long long>(row) * D + hf * 64 + t * 16) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <int D, int RT>
+__device__ __forceinline__ void load_v(Step<D, RT>& st, const uint8_t* v, int base, int n, int g, int t) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = base + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + 2 * t + (i & 1);
+    const uint8_t* at = v + static_cast<long long>(row) * D + g * (D / 8);
+    if (D == 128) {
+      const uint4 r = row < n ? load16(at) : make_uint4(0, 0, 0, 0);
+      st.v[i][0] = r.x;
+      st.v[i][1] = r.y;
+      st.v[i][D / 32 - 2] = r.z;
+      st.v[i][D / 32 - 1] = r.w;
+    } else {
+      uint2 r = make_uint2(0, 0);
+      if (row < n)
+        asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(at));
+      st.v[i][0] = r.x;
+      st.v[i][1] = r.y;
+    }
+  }
+}
+
+template <int D, int RT>
+__global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttnParams p) {
+  constexpr int R = RT * 8;         // query rows per item
+  constexpr int KS = D / 16;        // k-steps of the score product = m-tiles of the value product
+  __shared__ long long prefix[kMaxSeqs + 1];
+  __shared__ long long warp_sum[kWarps];
+  __shared__ float red[kWarps][R][D + 2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+
+  // ------------------------------------------------ the block list: prefix per sequence, this CTA's run
+  const long long heads = static_cast<long long>(p.Hkv) * p.row_groups;
+  long long base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kWarps * 32) {
+    const int b = b0 + tid;
+    long long n;
+    int first;
+    long long x = b < p.B ? seq_blocks(p, b, n, first) * heads : 0;
+    const long long own = x;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    long long before = base;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    for (int w = 0; w < kWarps; ++w) base += warp_sum[w];
+    if (b < p.B) prefix[b] = before + x - own;
+    __syncthreads();
+  }
+  const long long total = base;
+  if (tid == 0) prefix[p.B] = total;
+  __syncthreads();
+  long long run = (total + gridDim.x - 1) / gridDim.x;
+  run = run < kMinRun ? kMinRun : run;
+  if (blockIdx.x == 0) {
+    for (int b = tid; b <= p.B; b += kWarps * 32) p.plan[b] = prefix[b];
+    if (tid == 0) p.plan[p.B + 1] = run;
+  }
+  long long pos = blockIdx.x * run;
+  const long long end = min(pos + run, total);
+  if (pos >= end) return;
+  int b = 0;
+  {
+    int hi = p.B;  // last sequence with prefix <= pos (empty ones share a prefix with their follower)
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (prefix[mid] <= pos) b = mid;
+      else hi = mid;
+    }
+  }
+
+  while (pos < end) {
+    while (prefix[b + 1] <= pos) ++b;
+    long long n64;
+    int first;
+    const int nb = seq_blocks(p, b, n64, first);
+    const int n = static_cast<int>(n64);
+    const long long rel = pos - prefix[b];
+    const int hr = static_cast<int>(rel / nb);  // (KV head, row group)
+    const int j0 = static_cast<int>(rel - static_cast<long long>(hr) * nb);
+    const int j1 = static_cast<int>(min(static_cast<long long>(nb), j0 + (end - pos)));
+    const int hk = hr / p.row_groups;
+    const int row0 = (hr - hk * p.row_groups) * R;
+    const int rows = p.s * p.group;
+
+    // ---------------------------------------------- query rows: B fragments and row factors
+    uint32_t q[RT][KS][2];
+    float rf[RT][2];            // factor of rows 2t, 2t + 1: softmax scale, log2(e), the row's power of two
+    int kmax[RT][2], kmin[RT][2];
+    int lo_max = INT_MAX;        // lowest kmax and highest kmin of the item's rows: steps between need no mask
+    int hi_min = 0;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + rt * 8 + g;
+      float x[D / 4];
+      float amax = 0.f;
+      if (r < rows) {
+        const int i = r / p.group;
+        const __nv_bfloat16* src = p.q + b * p.q_sb + i * p.q_ss + (hk * p.group + r - i * p.group) * p.q_sh;
+#pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(src + hf * 64 + t * 16 + w * 8);
+            const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float lo = __uint_as_float(u[e] << 16), hi = __uint_as_float(u[e] & 0xffff0000u);
+              x[hf * 16 + w * 8 + 2 * e] = lo;
+              x[hf * 16 + w * 8 + 2 * e + 1] = hi;
+              amax = fmaxf(amax, fmaxf(fabsf(lo), fabsf(hi)));
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < D / 4; ++e) x[e] = 0.f;
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // 2^-k with amax in [2^k, 2^(k+1)); 1 for rows that are zero or not finite
+      const uint32_t ex = (__float_as_uint(amax) >> 23) & 255u;
+      const bool plain = ex < 2u || ex > 252u;
+      const float down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
+      const float up = plain ? 1.f : __uint_as_float(ex << 23);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        q[rt][ks][0] = pack_f16(x[4 * ks] * down, x[4 * ks + 1] * down);
+        q[rt][ks][1] = pack_f16(x[4 * ks + 2] * down, x[4 * ks + 3] * down);
+      }
+      const float f = up * p.scale_log2;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rf[rt][e] = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4);
+        const int rr = row0 + rt * 8 + 2 * t + e;
+        const int at = n - p.s + rr / p.group;  // the row's position
+        kmax[rt][e] = rr < rows ? at : -1;
+        kmin[rt][e] = p.window >= 0 ? max(at - p.window, 0) : 0;
+        if (rr < rows) {
+          lo_max = min(lo_max, at);
+          hi_min = max(hi_min, kmin[rt][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      lo_max = min(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, off));
+      hi_min = max(hi_min, __shfl_xor_sync(0xffffffffu, hi_min, off));
+    }
+
+    const uint8_t* kp = p.k + b * p.k_sb + hk * p.k_sh;
+    const uint8_t* vp = p.v + b * p.v_sb + hk * p.v_sh;
+    const float* ksp = p.k_scale + b * p.ks_sb + hk * p.ks_sh;
+    const float* vsp = p.v_scale + b * p.vs_sb + hk * p.vs_sh;
+
+    float m[RT][2], l[RT][2], o[RT][KS][4];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[rt][e] = -INFINITY;
+        l[rt][e] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[rt][mt][e] = 0.f;
+    }
+
+    Step<D, RT> st;
+    int j = j0 + warp;
+    if (j < j1) {
+      const int base_row = (first + j) * kCacheBlock;
+      st.ks = ksp[first + j];
+      st.vs = vsp[first + j];
+      load_k<D, RT>(st, kp, base_row, n, g, t);
+      load_v<D, RT>(st, vp, base_row, n, g, t);
+    }
+    for (; j < j1; j += kWarps) {
+      const int base_row = (first + j) * kCacheBlock;
+      const bool more = j + kWarps < j1;
+      const int next_row = base_row + kWarps * kCacheBlock;
+      const float ks_now = st.ks, vs_now = st.vs;
+      // ------------------------------------------ S^T = K Q^T
+      float s[RT][2][4];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[rt][mt][e] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf) {
+          const uint4 ra = st.k[2 * mt][hf], rb = st.k[2 * mt + 1][hf];
+          const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = f16x2_of(wa[w]), a2 = f16x2_of(wa[w] >> 16);
+            const uint32_t a1 = f16x2_of(wb[w]), a3 = f16x2_of(wb[w] >> 16);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) mma_f16(s[rt][mt], a0, a1, a2, a3, q[rt][hf * 4 + w][0], q[rt][hf * 4 + w][1]);
+          }
+        }
+      }
+      if (more) {
+        st.ks = ksp[first + j + kWarps];
+        st.vs = vsp[first + j + kWarps];
+        load_k<D, RT>(st, kp, next_row, n, g, t);
+      }
+      const bool edge = base_row + kCacheBlock - 1 > lo_max || base_row < hi_min;
+      if (edge) {
+        // A value row may hold NaN where only some rows see it: its bytes become zero, and the
+        // scores of the rows that do see it become NaN.
+        uint32_t bad = 0;  // bit i: key i of st.v has a NaN in this lane's channels
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) {
+            const uint32_t nb8 = nan_bytes(st.v[i][w]);
+            st.v[i][w] &= ~nb8;
+            any |= nb8;
+          }
+          bad |= any != 0 ? 1u << i : 0u;
+        }
+        uint32_t badrows = 0;  // bit per key of the step, over the whole warp
+        if (__any_sync(0xffffffffu, bad != 0)) {
+          uint32_t mine = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (bad >> i & 1) mine |= 1u << ((i >> 2) * 16 + ((i >> 1) & 1) * 8 + 2 * t + (i & 1));
+          badrows = __reduce_or_sync(0xffffffffu, mine);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int in = mt * 16 + (e >> 1) * 8 + g;
+              const int key = base_row + in;
+              if (badrows >> in & 1) s[rt][mt][e] = NAN;
+              if (key > kmax[rt][e & 1] || key < kmin[rt][e & 1]) s[rt][mt][e] = -INFINITY;
+            }
+      }
+      // ------------------------------------------ running maximum, P
+      uint32_t pf[RT][2][2];
+      float corr[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float f = rf[rt][e] * ks_now;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            // a hidden key stays -inf whatever the factor's sign or size
+            float& x0 = s[rt][mt][e];
+            float& x1 = s[rt][mt][e + 2];
+            x0 = x0 == -INFINITY ? x0 : x0 * f;
+            x1 = x1 == -INFINITY ? x1 : x1 * f;
+          }
+          float mx = fmaxf(fmaxf(s[rt][0][e], s[rt][0][e + 2]), fmaxf(s[rt][1][e], s[rt][1][e + 2]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[rt][e], mx);
+          corr[rt][e] = m[rt][e] == -INFINITY ? 0.f : exp2_fast(m[rt][e] - mn);
+          m[rt][e] = mn;
+          const float ref = mn == -INFINITY ? 0.f : mn - 10.f;
+          float add = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int hh = 0; hh < 4; hh += 2) {
+              const float x = exp2_fast(s[rt][mt][e + hh] - ref);
+              s[rt][mt][e + hh] = x;
+              add += x;
+            }
+          l[rt][e] = l[rt][e] * corr[rt][e] + add;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          pf[rt][mt][0] = transpose8x8(pack_f16(s[rt][mt][0], s[rt][mt][1]));
+          pf[rt][mt][1] = transpose8x8(pack_f16(s[rt][mt][2], s[rt][mt][3]));
+        }
+      }
+      // ------------------------------------------ O^T += V^T P^T, two m-tiles of channels per word
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) {
+        float c[RT][2][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[rt][x][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const uint32_t r0 = st.v[4 * ks][w], r1 = st.v[4 * ks + 1][w], r2 = st.v[4 * ks + 2][w],
+                         r3 = st.v[4 * ks + 3][w];
+          const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
+          const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
+          {
+            const uint32_t a0 = f16x2_of(lo01), a1 = f16x2_of(lo01 >> 16), a2 = f16x2_of(lo23), a3 = f16x2_of(lo23 >> 16);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) mma_f16(c[rt][0], a0, a1, a2, a3, pf[rt][ks][0], pf[rt][ks][1]);
+          }
+          {
+            const uint32_t a0 = f16x2_of(hi01), a1 = f16x2_of(hi01 >> 16), a2 = f16x2_of(hi23), a3 = f16x2_of(hi23 >> 16);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) mma_f16(c[rt][1], a0, a1, a2, a3, pf[rt][ks][0], pf[rt][ks][1]);
+          }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[rt][2 * w + x][e] = fmaf(o[rt][2 * w + x][e], corr[rt][e & 1], c[rt][x][e] * vs_now);
+      }
+      if (more) load_v<D, RT>(st, vp, next_row, n, g, t);
+    }
+
+    // ---------------------------------------------- merge the warps
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[rt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        float* dst = red[warp][rt * 8 + 2 * t + e];
+        // fragment (m-tile mt, half e2) of lane g is channel g * D / 8 + 2 mt + e2
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) {
+          dst[g * (D / 8) + 2 * mt] = o[rt][mt][e];
+          dst[g * (D / 8) + 2 * mt + 1] = o[rt][mt][e + 2];
+        }
+        if (g == 0) {
+          dst[D] = m[rt][e];
+          dst[D + 1] = x;
+        }
+      }
+    __syncthreads();
+    const bool whole = j0 == 0 && j1 == nb;
+    const long long item = b * heads + hr;
+    float* part = p.part + (blockIdx.x + item) * R * (D + 2);
+    for (int w = tid; w < R * (D / 4); w += kWarps * 32) {
+      const int r = w / (D / 4), c = (w - r * (D / 4)) * 4;
+      if (row0 + r >= rows) continue;
+      float M = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) M = fmaxf(M, red[x][r][D]);
+      float L = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float mw = red[x][r][D];
+        const float f = mw == -INFINITY && M != -INFINITY ? 0.f : (M == -INFINITY ? 1.f : exp2_fast(mw - M));
+        L += red[x][r][D + 1] * f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += red[x][r][c + e] * f;
+      }
+      if (whole) {
+        const int rr = row0 + r, i = rr / p.group;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const uint2 y = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
+        __nv_bfloat16* dst =
+            p.out + ((static_cast<long long>(b) * p.s + i) * p.H + hk * p.group + rr - i * p.group) * D + c;
+        *reinterpret_cast<uint2*>(dst) = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[r * (D + 2) + c + e] = a[e];
+        if (c == 0) {
+          part[r * (D + 2) + D] = M;
+          part[r * (D + 2) + D + 1] = L;
+        }
+      }
+    }
+    __syncthreads();  // red is written again for the next item
+    pos += j1 - j0;
+  }
+}
+
+// One warp per output row: the partials of the CTAs whose runs met its item, in their order.
+// Rows of items inside one run were written already; rows without a visible block become zero.
+template <int D>
+__global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnParams p, int R) {
+  const int lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (b, token, head)
+  if (row >= static_cast<long long>(p.B) * p.s * p.H) return;
+  const int h = static_cast<int>(row % p.H);
+  const long long bi = row / p.H;
+  const int i = static_cast<int>(bi % p.s);
+  const int b = static_cast<int>(bi / p.s);
+  const int hk = h / p.group;
+  const int rr = i * p.group + h - hk * p.group;
+  const int rg = rr / R, r = rr - rg * R;
+  const long long heads = static_cast<long long>(p.Hkv) * p.row_groups;
+  const long long run = p.plan[p.B + 1];
+  const long long nb = (p.plan[b + 1] - p.plan[b]) / heads;
+  const int hr = hk * p.row_groups + rg;
+  const long long from = p.plan[b] + hr * nb;
+  constexpr int N = D / 32;
+  float a[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) a[e] = 0.f;
+  float L = 0.f, M = -INFINITY;
+  if (nb > 0) {
+    const long long c0 = from / run, c1 = (from + nb - 1) / run;
+    if (c0 == c1) return;
+    const long long item = b * heads + hr;
+    const float* part = p.part + ((c0 + item) * R + r) * (D + 2);
+    const long long step = static_cast<long long>(R) * (D + 2);
+    const int n = static_cast<int>(c1 - c0 + 1);
+    for (int c = lane; c < n; c += 32) M = fmaxf(M, part[c * step + D]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+      const float* x = part + c * step;
+      const float mw = x[D];
+      const float f = M == -INFINITY ? 1.f : (mw == -INFINITY ? 0.f : exp2_fast(mw - M));
+      L += x[D + 1] * f;
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        const float2 y = *reinterpret_cast<const float2*>(x + lane * N + e);
+        a[e] = fmaf(y.x, f, a[e]);
+        a[e + 1] = fmaf(y.y, f, a[e + 1]);
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  __nv_bfloat16* dst = p.out + row * D + lane * N;
+#pragma unroll
+  for (int e = 0; e < N; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(a[e] * inv, a[e + 1] * inv);
+}
+
+template <int D, int RT>
+int ctas_per_sm() {
+  static int cached = 0;
+  if (cached == 0) {
+    int n = 0;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_attn_kernel<D, RT>, kWarps * 32, 0);
+    cached = n < 1 ? 1 : n;
+  }
+  return cached;
+}
+
+int row_tiles(const CacheAttnParams& p) { return p.s * p.group <= 8 ? 1 : 2; }
+
+}  // namespace
+
+int cache_attn_max_seqs() { return kMaxSeqs; }
+
+void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long long* plan_words) {
+  const int rt = row_tiles(p), R = rt * 8;
+  p.row_groups = (p.s * p.group + R - 1) / R;
+  const int per_sm = D == 64 ? (rt == 1 ? ctas_per_sm<64, 1>() : ctas_per_sm<64, 2>())
+                             : (rt == 1 ? ctas_per_sm<128, 1>() : ctas_per_sm<128, 2>());
+  const long long items = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
+  const long long most = items * ((p.T + kCacheBlock - 1) / kCacheBlock);  // key blocks if all caches were full
+  const long long want = (most + kMinRun - 1) / kMinRun;
+  const long long full = static_cast<long long>(device_sm_count()) * per_sm;
+  p.grid = static_cast<int>(want < 1 ? 1 : (want < full ? want : full));
+  *part_floats = (p.grid + items) * R * (D + 2);
+  *plan_words = p.B + 2;
+}
+
+void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
+  const int rt = row_tiles(p);
+  const long long rows = static_cast<long long>(p.B) * p.s * p.H;
+  const unsigned merge = static_cast<unsigned>((rows + 3) / 4);
+  if (D == 64) {
+    if (rt == 1)
+      cache_attn_kernel<64, 1><<<p.grid, kWarps * 32, 0, stream>>>(p);
+    else
+      cache_attn_kernel<64, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
+    cache_attn_merge_kernel<64><<<merge, 128, 0, stream>>>(p, rt * 8);
+  } else {
+    if (rt == 1)
+      cache_attn_kernel<128, 1><<<p.grid, kWarps * 32, 0, stream>>>(p);
+    else
+      cache_attn_kernel<128, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
+    cache_attn_merge_kernel<128><<<merge, 128, 0, stream>>>(p, rt * 8);
+  }
+}
+
+}  // namespace pb

@@ -366,4 +366,81 @@ void gdn_chunk_fwd(const void* w, const void* qg, const void* mqk, const void* k
 void gdn_chunk_bwd(const void* kr, const void* mqk, const void* dout, const void* qg, const void* w,
                    const GdnParams& p, cudaStream_t stream);
 
+// Rotary embedding of q [B, S, H, D] and k [B, S, Hk, D] (any strides, contiguous channels) in one
+// launch (rotary.cu). Factors: fp32 rows of R / 2 with element strides per batch, token and head
+// (0 where shared). Outputs contiguous. dtype: 0 bf16, 1 fp32, 2 fp16.
+struct RotaryParams {
+  const void* q;
+  const void* k;
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh;
+  void* q_out;
+  void* k_out;
+  const float* cos;
+  const float* sin;
+  long long f_sb, f_ss, f_sh;
+  long long tokens;  // B * S
+  int S, H, Hk, D, R;
+  float sign;        // -1: the transposed rotation (the gradient)
+  int interleave;
+  int tokens_per_block;  // set by the launcher
+};
+void rotary(RotaryParams p, int dtype, cudaStream_t stream);
+
+// 8-bit caches: e4m3 rows with one power-of-two scale per kCacheBlock rows and head.
+constexpr int kCacheBlock = 32;
+constexpr int kCacheMinExp = -100;
+constexpr int kCacheMaxExp = 120;
+
+// Rotates s tokens per sequence at positions lengths[b] + i (cos / sin: fp32 [table_rows, R / 2],
+// or null for no rotation and no q output) and appends keys and values to the 8-bit caches
+// [B, Hkv, T, D] (contiguous rows) with scales [B, Hkv, ceil(T / 32)] (rotary.cu).
+struct AppendParams {
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+  __nv_bfloat16* q_out;  // [B, s, H, D]
+  const float* cos;
+  const float* sin;
+  long long table_rows;
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  long long kc_sb, kc_sh, vc_sb, vc_sh;
+  float* k_scale;
+  float* v_scale;
+  long long ks_sb, ks_sh, vs_sb, vs_sh;
+  const int* lengths;
+  int B, s, H, Hkv, T, R;
+  long long q_blocks;   // set by the launcher
+  int blocks_per_seq;   // set by the launcher
+};
+void rotary_append(AppendParams p, int D, bool interleave, cudaStream_t stream);
+
+// Attention of s query tokens per sequence over the 8-bit caches (cache_attention.cu). Query i of
+// sequence b stands at position n - s + i with n = min(lengths[b] + offset, T) and sees the keys at
+// or before it, not more than `window` behind it (window >= 0).
+struct CacheAttnParams {
+  const __nv_bfloat16* q;  // [B, s, H, D], contiguous channels
+  long long q_sb, q_ss, q_sh;
+  const uint8_t* k;        // [B, Hkv, T, D] e4m3, contiguous rows
+  const uint8_t* v;
+  long long k_sb, k_sh, v_sb, v_sh;
+  const float* k_scale;    // [B, Hkv, ceil(T / 32)]
+  const float* v_scale;
+  long long ks_sb, ks_sh, vs_sb, vs_sh;
+  const int* lengths;
+  __nv_bfloat16* out;      // [B, s, H, D] contiguous
+  int B, s, H, Hkv, T, group, offset, window;
+  float scale_log2;        // softmax scale * log2(e)
+  // workspace of the split form (sizes from cache_attn_plan)
+  float* part;             // [slots, rows, D + 2]
+  long long* plan;         // [B + 2] block prefix per sequence, total, blocks per CTA
+  int row_groups, grid;
+  int* status;
+};
+// Rows (s * group) per work item, CTAs and workspace slots of the split form.
+int cache_attn_max_seqs();  // sequences per launch at most
+void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long long* plan_words);
+void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream);
+
 }  // namespace pb

@@ -1,0 +1,352 @@
+// Rotary embedding in every layout the models use, and the append of rotated keys and of
+// values to an 8-bit cache.
+//
+// Rotation. A head's first R channels hold R / 2 pairs (a, c): channels (i, i + R/2) in the
+// half-split layout, (2i, 2i + 1) in the interleaved one. With the factors (cos, sin) of the
+// token's position the pair becomes
+//   a' = a cos - c sin        c' = c cos + a sin
+// and channels R..D-1 are copied. Every product and sum is rounded separately in fp32 (no
+// FMA), as torch's elementwise operations round them, so both orders give the same bits; the
+// result is rounded once to the tensor's type. The factors may carry a length-scaling
+// magnitude. The gradient is the same kernel with -sin.
+//
+// Append. Rows of keys (rotated, still fp32) and values are stored as e4m3 with one scale
+// 2^e per (sequence, head, 32 cache rows): e is the least with amax / 2^e <= 448, so dividing
+// by the scale is exact and each value is rounded once. A block that already holds rows
+// keeps max(e_old, e_new); when e grows its old rows are requantised by the exact factor
+// 2^(e_old - e). Values that are not finite are stored as NaN and do not take part in amax.
+//
+// Both are bound by their bytes: each value is read and written once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace pb {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+__device__ __forceinline__ void turn(float a, float c, float cs, float sn, float& ya, float& yc) {
+  ya = __fsub_rn(__fmul_rn(a, cs), __fmul_rn(c, sn));
+  yc = __fadd_rn(__fmul_rn(c, cs), __fmul_rn(a, sn));
+}
+
+// One thread turns (or copies) 2 V channels of one head: two vectors of V elements each.
+// Units of a head: R / (2V) turned ones, then (D - R) / (2V) copied ones.
+template <typename T, int V, bool INTER>
+__global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
+  const int units = p.D / (2 * V);
+  const int turned = p.R / (2 * V);
+  const int heads = p.H + p.Hk;
+  const int per_token = heads * units;
+  const long long tok0 = static_cast<long long>(blockIdx.x) * p.tokens_per_block;
+  const int ntok = static_cast<int>(min(static_cast<long long>(p.tokens_per_block), p.tokens - tok0));
+  for (int w = threadIdx.x; w < ntok * per_token; w += blockDim.x) {
+    const int lt = w / per_token;
+    const int r = w - lt * per_token;
+    const int h = r / units;
+    const int u = r - h * units;
+    const long long tok = tok0 + lt;
+    const long long b = tok / p.S;
+    const long long s = tok - b * p.S;
+    const bool is_q = h < p.H;
+    const int hh = is_q ? h : h - p.H;
+    const T* src = is_q ? static_cast<const T*>(p.q) + b * p.q_sb + s * p.q_ss + hh * p.q_sh
+                        : static_cast<const T*>(p.k) + b * p.k_sb + s * p.k_ss + hh * p.k_sh;
+    T* dst = is_q ? static_cast<T*>(p.q_out) + (tok * p.H + hh) * p.D : static_cast<T*>(p.k_out) + (tok * p.Hk + hh) * p.D;
+    int e0, e1;  // first channels of the thread's two vectors
+    if (u >= turned) {
+      e0 = p.R + (u - turned) * 2 * V;
+      e1 = e0 + V;
+    } else if (INTER) {
+      e0 = u * 2 * V;
+      e1 = e0 + V;
+    } else {
+      e0 = u * V;
+      e1 = e0 + p.R / 2;
+    }
+    const Vec<T, V> x0 = *reinterpret_cast<const Vec<T, V>*>(src + e0);
+    const Vec<T, V> x1 = *reinterpret_cast<const Vec<T, V>*>(src + e1);
+    Vec<T, V> y0 = x0, y1 = x1;
+    if (u < turned) {
+      const long long at = b * p.f_sb + s * p.f_ss + (p.f_sh == 0 ? 0 : hh * p.f_sh) + u * V;
+      float cs[V], sn[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        cs[i] = p.cos[at + i];
+        sn[i] = p.sign * p.sin[at + i];
+      }
+      if (INTER) {
+        // pair i of the unit: channels 2i and 2i + 1 of its 2V contiguous ones
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float a = to_f(2 * i < V ? x0.v[(2 * i) % V] : x1.v[(2 * i) % V]);
+          const float c = to_f(2 * i + 1 < V ? x0.v[(2 * i + 1) % V] : x1.v[(2 * i + 1) % V]);
+          float ya, yc;
+          turn(a, c, cs[i], sn[i], ya, yc);
+          if (2 * i < V)
+            y0.v[(2 * i) % V] = from_f<T>(ya);
+          else
+            y1.v[(2 * i) % V] = from_f<T>(ya);
+          if (2 * i + 1 < V)
+            y0.v[(2 * i + 1) % V] = from_f<T>(yc);
+          else
+            y1.v[(2 * i + 1) % V] = from_f<T>(yc);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float ya, yc;
+          turn(to_f(x0.v[i]), to_f(x1.v[i]), cs[i], sn[i], ya, yc);
+          y0.v[i] = from_f<T>(ya);
+          y1.v[i] = from_f<T>(yc);
+        }
+      }
+    }
+    *reinterpret_cast<Vec<T, V>*>(dst + e0) = y0;
+    *reinterpret_cast<Vec<T, V>*>(dst + e1) = y1;
+  }
+}
+
+template <typename T, int V>
+void launch_rotary_v(RotaryParams& p, cudaStream_t stream) {
+  const int per_token = (p.H + p.Hk) * (p.D / (2 * V));
+  p.tokens_per_block = per_token >= 256 ? 1 : 256 / per_token;
+  const long long blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+  if (p.interleave)
+    rotary_kernel<T, V, true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+  else
+    rotary_kernel<T, V, false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+}
+
+// Widest vector that the channel counts, strides and base addresses all allow.
+template <typename T>
+void launch_rotary(RotaryParams& p, cudaStream_t stream) {
+  auto fits = [&](int v) {
+    const long long bytes = static_cast<long long>(v) * sizeof(T);
+    if (p.D % (2 * v) != 0 || p.R % (2 * v) != 0) return false;
+    for (const void* a : {p.q, p.k, static_cast<const void*>(p.q_out), static_cast<const void*>(p.k_out)})
+      if (reinterpret_cast<uintptr_t>(a) % bytes != 0) return false;
+    for (long long st : {p.q_sb, p.q_ss, p.q_sh, p.k_sb, p.k_ss, p.k_sh})
+      if (st % v != 0) return false;
+    return true;
+  };
+  constexpr int kWide = 16 / sizeof(T);
+  if (fits(kWide))
+    launch_rotary_v<T, kWide>(p, stream);
+  else if (kWide > 4 && fits(4))
+    launch_rotary_v<T, 4>(p, stream);
+  else if (fits(2))
+    launch_rotary_v<T, 2>(p, stream);
+  else
+    launch_rotary_v<T, 1>(p, stream);
+}
+
+// ------------------------------------------------------------------------------- append
+constexpr int kRows = kCacheBlock;  // cache rows per scale
+constexpr int kThreads = 128;
+
+// Least power of two s with amax / s <= 448 = 1.75 * 2^8, from amax's exponent and mantissa.
+__device__ __forceinline__ float block_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = min(max(e, kCacheMinExp), kCacheMaxExp);
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t e4m3_of(float x) {
+  const uint32_t u = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  return fabsf(x) < INFINITY ? u : 0x7fu;
+}
+
+__device__ __forceinline__ float of_e4m3(uint32_t byte) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+
+// The lane's N = D / 32 channels of one row, turned in fp32 when `cs` is given (the row's factors).
+template <int N, bool INTER>
+__device__ __forceinline__ void load_turned(const __nv_bfloat16* row, int lane, int R, const float* cs, const float* sn,
+                                            float (&x)[N]) {
+  const int e0 = lane * N;
+  const Vec<__nv_bfloat16, N> raw = *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(row + e0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = to_f(raw.v[i]);
+  if (cs == nullptr || e0 >= R) return;
+  if (INTER) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      if (e0 + i < R) {
+        const int f = (e0 + i) >> 1;
+        float ya, yc;
+        turn(x[i], x[i + 1], cs[f], sn[f], ya, yc);
+        x[i] = ya;
+        x[i + 1] = yc;
+      }
+    }
+  } else {
+    const int half = R >> 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = e0 + i;
+      if (e < R) {
+        const bool first = e < half;
+        const int f = first ? e : e - half;
+        const float other = to_f(row[first ? e + half : e - half]);
+        float ya, yc;
+        turn(first ? x[i] : other, first ? other : x[i], cs[f], sn[f], ya, yc);
+        x[i] = first ? ya : yc;
+      }
+    }
+  }
+}
+
+// CTAs [0, q_blocks) turn the queries, one token each (its heads over the four warps). The rest
+// take one (sequence, KV head, block of 32 cache rows, K or V) each: pass one leaves the rows'
+// values in registers and finds amax, pass two requantises old rows if need be and stores.
+template <int D, bool INTER>
+__global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p) {
+  constexpr int N = D / 32;
+  constexpr int kWarpRows = kRows / (kThreads / 32);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  long long blk = blockIdx.x;
+  if (blk < p.q_blocks) {
+    const long long b = blk / p.s;
+    const int i = static_cast<int>(blk - b * p.s);
+    const long long pos = min(max(static_cast<long long>(p.lengths[b]) + i, 0LL), p.table_rows - 1);
+    const float* cs = p.cos + pos * (p.R >> 1);
+    const float* sn = p.sin + pos * (p.R >> 1);
+    const __nv_bfloat16* src = p.q + b * p.q_sb + i * p.q_ss;
+    __nv_bfloat16* dst = p.q_out + blk * p.H * D;
+#pragma unroll 4
+    for (int h = warp; h < p.H; h += kThreads / 32) {
+      float x[N];
+      load_turned<N, INTER>(src + h * p.q_sh, lane, p.R, cs, sn, x);
+      Vec<__nv_bfloat16, N> y;
+#pragma unroll
+      for (int j = 0; j < N; ++j) y.v[j] = from_f<__nv_bfloat16>(x[j]);
+      *reinterpret_cast<Vec<__nv_bfloat16, N>*>(dst + h * D + lane * N) = y;
+    }
+    return;
+  }
+  blk -= p.q_blocks;
+  const bool is_v = blk & 1;
+  blk >>= 1;
+  const int nth = static_cast<int>(blk % p.blocks_per_seq);
+  blk /= p.blocks_per_seq;
+  const int hk = static_cast<int>(blk % p.Hkv);
+  const long long b = blk / p.Hkv;
+  const long long start = p.lengths[b];               // first appended row
+  const long long end = min(start + p.s, static_cast<long long>(p.T));
+  if (start < 0) return;
+  const long long cb = start / kRows + nth;           // cache block
+  const long long row0 = cb * kRows;
+  const int lo = static_cast<int>(max(start - row0, 0LL));          // appended rows of the block: [lo, hi)
+  const int hi = static_cast<int>(min(end - row0, static_cast<long long>(kRows)));
+  if (hi <= lo) return;
+
+  const __nv_bfloat16* x0 = is_v ? p.v + b * p.v_sb + hk * p.v_sh : p.k + b * p.k_sb + hk * p.k_sh;
+  const long long x_ss = is_v ? p.v_ss : p.k_ss;
+  uint8_t* cache = (is_v ? p.v_cache + b * p.vc_sb + hk * p.vc_sh : p.k_cache + b * p.kc_sb + hk * p.kc_sh) + row0 * D;
+  float* scale = (is_v ? p.v_scale + b * p.vs_sb + hk * p.vs_sh : p.k_scale + b * p.ks_sb + hk * p.ks_sh) + cb;
+  const bool turn_it = !is_v && p.cos != nullptr;
+
+  float x[kWarpRows][N];
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < kWarpRows; ++j) {
+    const int r = warp + j * (kThreads / 32);
+    if (r >= lo && r < hi) {
+      const long long pos = min(row0 + r, p.table_rows - 1);
+      load_turned<N, INTER>(x0 + (row0 + r - start) * x_ss, lane, p.R, turn_it ? p.cos + pos * (p.R >> 1) : nullptr,
+                            turn_it ? p.sin + pos * (p.R >> 1) : nullptr, x[j]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float a = fabsf(x[j][i]);
+        if (a < INFINITY) amax = fmaxf(amax, a);  // false for NaN too
+      }
+    }
+  }
+  const float held = lo > 0 ? *scale : 0.f;  // read before the barrier below, written after it
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  __shared__ float red[kThreads / 32];
+  if (lane == 0) red[warp] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, red[w]);
+  const float now = fmaxf(block_scale(amax), held);
+  const float inv = 1.f / now;
+  if (threadIdx.x == 0) *scale = now;
+#pragma unroll
+  for (int j = 0; j < kWarpRows; ++j) {
+    const int r = warp + j * (kThreads / 32);
+    if (r >= lo && r < hi) {
+      Vec<uint8_t, N> y;
+#pragma unroll
+      for (int i = 0; i < N; ++i) y.v[i] = static_cast<uint8_t>(e4m3_of(x[j][i] * inv));
+      *reinterpret_cast<Vec<uint8_t, N>*>(cache + r * D + lane * N) = y;
+    } else if (r < lo && now > held) {
+      Vec<uint8_t, N>* at = reinterpret_cast<Vec<uint8_t, N>*>(cache + r * D + lane * N);
+      Vec<uint8_t, N> y = *at;
+      const float f = held * inv;
+#pragma unroll
+      for (int i = 0; i < N; ++i) y.v[i] = static_cast<uint8_t>(e4m3_of(of_e4m3(y.v[i]) * f));
+      *at = y;
+    }
+  }
+}
+
+}  // namespace
+
+void rotary(RotaryParams p, int dtype, cudaStream_t stream) {
+  if (dtype == 0)
+    launch_rotary<__nv_bfloat16>(p, stream);
+  else if (dtype == 1)
+    launch_rotary<float>(p, stream);
+  else
+    launch_rotary<__half>(p, stream);
+}
+
+void rotary_append(AppendParams p, int D, bool interleave, cudaStream_t stream) {
+  p.q_blocks = p.cos != nullptr ? static_cast<long long>(p.B) * p.s : 0;
+  p.blocks_per_seq = p.s == 1 ? 1 : (p.s - 1 + kRows - 1) / kRows + 1;
+  const long long blocks = p.q_blocks + 2LL * p.B * p.Hkv * p.blocks_per_seq;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (D == 64) {
+    if (interleave)
+      rotary_append_kernel<64, true><<<grid, kThreads, 0, stream>>>(p);
+    else
+      rotary_append_kernel<64, false><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    if (interleave)
+      rotary_append_kernel<128, true><<<grid, kThreads, 0, stream>>>(p);
+    else
+      rotary_append_kernel<128, false><<<grid, kThreads, 0, stream>>>(p);
+  }
+}
+
+}  // namespace pb

@@ -407,6 +407,54 @@ class _Rotary(torch.autograd.Function):
         return n.rope(dq.contiguous(), c, s, -1.0), n.rope(dk.contiguous(), c, s, -1.0), None, None
 
 
+class _RotaryAny(torch.autograd.Function):
+    """Either pair layout, part of the head, factors per sequence or per head (``csrc/rotary.cu``).
+
+    The rotation is linear, and its transpose is the rotation by ``-sin``: the backward is this function again.
+    """
+
+    @staticmethod
+    def forward(ctx, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, interleave: bool, sign: float):  # type: ignore[override]
+        ctx.save_for_backward(cos, sin)
+        ctx.interleave, ctx.sign = interleave, sign
+        q, k = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k))
+        return tuple(native().rotary(q, k, cos, sin, interleave, sign))
+
+    @staticmethod
+    def backward(ctx, dq: Tensor, dk: Tensor):  # type: ignore[override]
+        cos, sin = ctx.saved_tensors
+        return *_RotaryAny.apply(dq, dk, cos, sin, ctx.interleave, -ctx.sign), None, None, None, None
+
+
+def rotary_any_supported(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> bool:
+    """Shapes and types that :class:`_RotaryAny` covers (factors that need a gradient do not)."""
+    return (
+        q.ndim == 4
+        and k.ndim == 4
+        and q.is_cuda
+        and q.device == k.device
+        and q.dtype == k.dtype
+        and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
+        and q.shape[:2] == k.shape[:2]
+        and q.shape[-1] == k.shape[-1]
+        and q.shape[0] * q.shape[1] < 1 << 31
+        and (q.shape[2] + k.shape[2]) * q.shape[3] < 1 << 22
+        and cos.shape == sin.shape
+        and cos.is_floating_point()
+        and cos.dtype != torch.float64
+        and cos.ndim in (3, 4)
+        and 2 <= 2 * cos.shape[-1] <= q.shape[-1]
+        and cos.shape[-3] == q.shape[1]
+        and (cos.ndim == 3 or cos.shape[0] in (1, q.shape[0]))
+        and (cos.shape[-2] == 1 or cos.shape[-2] == q.shape[2] == k.shape[2])
+        and not (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad))
+    )
+
+
+def rotary_any(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, interleave: bool) -> tuple[Tensor, Tensor]:
+    return _RotaryAny.apply(q, k, cos.float(), sin.float(), interleave, 1.0)
+
+
 def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> tuple[Tensor, Tensor]:
     if q.shape[-1] % 4 != 0 or cos.requires_grad or sin.requires_grad:
         from priml_b200.ops import reference

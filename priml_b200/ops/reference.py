@@ -36,6 +36,21 @@ def rotate_half(x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
     return torch.cat([x0 * cos - x1 * sin, x1 * cos + x0 * sin], dim=-1).to(dtype)
 
 
+def rotate(x: Tensor, cos: Tensor, sin: Tensor, interleave: bool = False) -> Tensor:
+    """Rotation of the first ``2 * cos.shape[-1]`` channels of ``[..., S, H, D]`` in fp32, rounded once.
+
+    The pairs are channels ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleave``; the others are copied.
+    """
+    rot = 2 * cos.shape[-1]
+    if rot > x.shape[-1]:
+        raise ValueError(f"{rot} rotated channels do not fit {x.shape[-1]} channels.")
+    turned, rest = x[..., :rot].float(), x[..., rot:]
+    a, c = (turned[..., 0::2], turned[..., 1::2]) if interleave else turned.chunk(2, dim=-1)
+    pair = (a * cos - c * sin, c * cos + a * sin)
+    y = torch.stack(pair, dim=-1).flatten(-2) if interleave else torch.cat(pair, dim=-1)
+    return torch.cat([y.to(x.dtype), rest], dim=-1) if rest.shape[-1] else y.to(x.dtype)
+
+
 def attention(
     q: Tensor,
     k: Tensor,
@@ -95,6 +110,110 @@ def decode_attention(
     s = s.masked_fill(~ok[:, None, :], float("-inf"))
     p = torch.nan_to_num(s.softmax(dim=-1), nan=0.0)  # an empty row gives zeros
     return torch.einsum("bht,bhtd->bhd", p, vf).to(q.dtype)
+
+
+CACHE_BLOCK = 32
+"""Cache rows of one head that share a scale."""
+
+
+def cache_scale(amax: Tensor) -> Tensor:
+    """The least power of two ``p`` in [2**-100, 2**120] with ``amax / p <= 448``, e4m3's largest value."""
+    mant, exp = torch.frexp(amax.float())  # amax = mant * 2**exp, mant in [0.5, 1); 448 = 0.875 * 2**9
+    exp = exp - 9 + (mant > 0.875).to(exp.dtype)
+    exp = torch.where(amax > 0, exp, torch.full_like(exp, -100)).clamp(-100, 120)
+    return torch.ldexp(torch.ones_like(mant), exp)
+
+
+def _to_e4m3(x: Tensor) -> Tensor:
+    return torch.where(x.isfinite(), x, torch.full_like(x, float("nan"))).to(torch.float8_e4m3fn)
+
+
+def cache_append(x: Tensor, cache: Tensor, scale: Tensor, lengths: Tensor) -> None:
+    """Quantise ``[B, s, Hkv, D]`` rows into rows ``lengths[b] + i`` of an 8-bit cache ``[B, Hkv, T, D]``.
+
+    A block of 32 rows that held rows before keeps its scale unless the new rows need a larger one, in
+    which case its old rows are requantised. Values that are not finite are stored as NaN and do not
+    enter the scale. Rows at or past ``T`` are dropped; a negative length appends nothing.
+    """
+    s, t = x.shape[1], cache.shape[2]
+    bits = cache.view(torch.uint8)
+    for b, start in enumerate(lengths.tolist()):
+        end = min(start + s, t)
+        for lo in range(start, end) if start >= 0 else ():
+            if lo != start and lo % CACHE_BLOCK:
+                continue  # the first row of each block that the rows [start, end) touch
+            block = lo // CACHE_BLOCK
+            first, hi = block * CACHE_BLOCK, min((block + 1) * CACHE_BLOCK, end)
+            rows = x[b, lo - start : hi - start].transpose(0, 1).float()  # [Hkv, rows, D]
+            size = torch.where(rows.isfinite(), rows.abs(), torch.zeros_like(rows)).amax((1, 2))
+            now = cache_scale(size)
+            if lo > first:
+                now = torch.maximum(now, scale[b, :, block])
+                held = cache[b, :, first:lo].float() * (scale[b, :, block] / now)[:, None, None]
+                bits[b, :, first:lo] = _to_e4m3(held).view(torch.uint8)
+            bits[b, :, lo:hi] = _to_e4m3(rows / now[:, None, None]).view(torch.uint8)
+            scale[b, :, block] = now
+
+
+def rotary_append(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    k_cache: Tensor,
+    v_cache: Tensor,
+    k_scale: Tensor,
+    v_scale: Tensor,
+    lengths: Tensor,
+    cos: Tensor | None,
+    sin: Tensor | None,
+    interleave: bool,
+) -> Tensor:
+    """Oracle of :func:`priml_b200.ops.rotary_append`: the keys go to the cache from the fp32 rotation."""
+    kf = k.float()
+    if cos is not None and sin is not None:
+        at = (lengths.long()[:, None] + torch.arange(q.shape[1], device=q.device)).clamp(0, cos.shape[0] - 1)
+        c, n = cos.float()[at][:, :, None], sin.float()[at][:, :, None]
+        q, kf = rotate(q, c, n, interleave), rotate(kf, c, n, interleave)
+    cache_append(kf, k_cache, k_scale, lengths)
+    cache_append(v.float(), v_cache, v_scale, lengths)
+    return q
+
+
+def cache_attention(
+    q: Tensor,
+    k_cache: Tensor,
+    v_cache: Tensor,
+    k_scale: Tensor,
+    v_scale: Tensor,
+    lengths: Tensor,
+    *,
+    scale: float,
+    window: int | None = None,
+    offset: int = 0,
+) -> Tensor:
+    """fp32 oracle of attention over an 8-bit cache: ``[B, s, H, D]`` queries, the last ``s`` tokens of each sequence."""
+    b, s, h, d = q.shape
+    hkv, t = k_cache.shape[1], k_cache.shape[2]
+    k, v = (
+        c.float() * f.repeat_interleave(CACHE_BLOCK, dim=2)[:, :, :t, None] for c, f in ((k_cache, k_scale), (v_cache, v_scale))
+    )
+    n = (lengths.to(device=q.device, dtype=torch.long) + offset).clamp(0, t)
+    pos = n[:, None] - s + torch.arange(s, device=q.device)
+    key = torch.arange(t, device=q.device)
+    ok = key <= pos[..., None]  # [B, s, T]
+    if window is not None:
+        ok &= key >= pos[..., None] - window
+    # rows that no query sees may hold anything
+    v = torch.where(ok.any(1)[:, None, :, None], v, torch.zeros_like(v))
+    qf = q.float().reshape(b, s, hkv, h // hkv, d)
+    z = torch.einsum("bskgd,bktd->bkgst", qf, k) * scale
+    z = z.masked_fill(~ok[:, None, None], float("-inf"))
+    p = torch.where(ok.any(-1)[:, None, None, :, None], z.softmax(dim=-1), torch.zeros_like(z))
+    bad = v.isnan()
+    o = torch.einsum("bkgst,bktd->bskgd", p, v.masked_fill(bad, 0.0))
+    if bool(bad.any()):  # a NaN reaches the queries that see its row, and no others
+        o = o.masked_fill(torch.einsum("bst,bktd->bskd", ok.float(), bad.float())[:, :, :, None] > 0, float("nan"))
+    return o.reshape(b, s, h, d).to(q.dtype)
 
 
 def mla_decode(
