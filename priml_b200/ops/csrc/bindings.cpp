@@ -883,34 +883,40 @@ Tensor cache_attn(const Tensor& q_, const Tensor& k, const Tensor& v, const Tens
   auto out = torch::empty({B, s, H, D}, q.options());
   if (out.numel() == 0) return out;
   if (T == 0) return out.zero_();
-  const int64_t step = pb::cache_attn_max_seqs();
-  for (int64_t b0 = 0; b0 < B; b0 += step) {
-    const int64_t nb = std::min(step, B - b0);
-    pb::CacheAttnParams p{};
-    p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()) + b0 * q.stride(0);
-    p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
-    p.k = static_cast<const uint8_t*>(k.data_ptr()) + b0 * k.stride(0);
-    p.v = static_cast<const uint8_t*>(v.data_ptr()) + b0 * v.stride(0);
-    p.k_sb = k.stride(0), p.k_sh = k.stride(1), p.v_sb = v.stride(0), p.v_sh = v.stride(1);
-    p.k_scale = k_scale.data_ptr<float>() + b0 * k_scale.stride(0);
-    p.v_scale = v_scale.data_ptr<float>() + b0 * v_scale.stride(0);
-    p.ks_sb = k_scale.stride(0), p.ks_sh = k_scale.stride(1);
-    p.vs_sb = v_scale.stride(0), p.vs_sh = v_scale.stride(1);
-    p.lengths = lengths.data_ptr<int>() + b0;
-    p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()) + b0 * s * H * D;
-    p.B = static_cast<int>(nb), p.s = static_cast<int>(s), p.H = static_cast<int>(H), p.Hkv = static_cast<int>(Hkv);
-    p.T = static_cast<int>(T), p.group = static_cast<int>(H / Hkv);
-    p.offset = static_cast<int>(offset);
-    p.window = static_cast<int>(std::min<int64_t>(window, T));
-    p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-    p.status = status_ptr();
-    long long part_floats = 0, plan_words = 0;
-    pb::cache_attn_plan(p, static_cast<int>(D), &part_floats, &plan_words);
-    auto part = torch::empty({part_floats}, q.options().dtype(torch::kFloat32));
-    auto plan = torch::empty({plan_words}, q.options().dtype(torch::kInt64));
-    p.part = part.data_ptr<float>();
-    p.plan = reinterpret_cast<long long*>(plan.data_ptr<int64_t>());
-    pb::cache_attn(p, static_cast<int>(D), stream());
+  pb::CacheAttnParams p{};
+  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+  p.k_sb = k.stride(0), p.k_sh = k.stride(1), p.v_sb = v.stride(0), p.v_sh = v.stride(1);
+  p.ks_sb = k_scale.stride(0), p.ks_sh = k_scale.stride(1);
+  p.vs_sb = v_scale.stride(0), p.vs_sh = v_scale.stride(1);
+  p.o_sb = s * H * D;
+  p.s = static_cast<int>(s), p.H = static_cast<int>(H), p.Hkv = static_cast<int>(Hkv);
+  p.T = static_cast<int>(T), p.group = static_cast<int>(H / Hkv);
+  p.offset = static_cast<int>(offset);
+  p.window = static_cast<int>(std::min<int64_t>(window, T));
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.status = status_ptr();
+  int seqs = 0, tokens = 0;
+  pb::cache_attn_limits(p, &seqs, &tokens);
+  for (int64_t b0 = 0; b0 < B; b0 += seqs) {
+    for (int64_t s0 = 0; s0 < s; s0 += tokens) {
+      p.B = static_cast<int>(std::min<int64_t>(seqs, B - b0));
+      p.s = static_cast<int>(std::min<int64_t>(tokens, s - s0));
+      p.back = static_cast<int>(s - s0 - p.s);
+      p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()) + b0 * q.stride(0) + s0 * q.stride(1);
+      p.k = static_cast<const uint8_t*>(k.data_ptr()) + b0 * k.stride(0);
+      p.v = static_cast<const uint8_t*>(v.data_ptr()) + b0 * v.stride(0);
+      p.k_scale = k_scale.data_ptr<float>() + b0 * k_scale.stride(0);
+      p.v_scale = v_scale.data_ptr<float>() + b0 * v_scale.stride(0);
+      p.lengths = lengths.data_ptr<int>() + b0;
+      p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()) + (b0 * s + s0) * H * D;
+      long long part_floats = 0, plan_words = 0;
+      pb::cache_attn_plan(p, static_cast<int>(D), &part_floats, &plan_words);
+      auto part = torch::empty({part_floats}, q.options().dtype(torch::kFloat32));
+      auto plan = torch::empty({plan_words}, q.options().dtype(torch::kInt64));
+      p.part = part.data_ptr<float>();
+      p.plan = reinterpret_cast<long long*>(plan.data_ptr<int64_t>());
+      pb::cache_attn(p, static_cast<int>(D), stream());
+    }
   }
   return out;
 }

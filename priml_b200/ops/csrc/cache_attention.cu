@@ -27,8 +27,8 @@
 // Work split: the key blocks of all (sequence, KV head, row group) items form one list, cut into
 // equal runs over the grid on the device from the lengths, so ragged batches load all SMs alike
 // and nothing depends on the host knowing a length. A run's piece of an item is written as an
-// unnormalised partial (slot = CTA + item: both only grow along the list, so slots are unique);
-// an item inside one run is finished at once. A second kernel merges the partials in slot order.
+// unnormalised partial (slot 2 CTA + 1 where the item begins in the run, 2 CTA where it began before);
+// an item inside one run is finished at once. A second kernel merges the partials in CTA order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -103,7 +103,8 @@ struct Item {
 // Keys of sequence b (0 .. T) and its visible key blocks.
 __device__ __forceinline__ int seq_blocks(const CacheAttnParams& p, int b, long long& n, int& first) {
   n = static_cast<long long>(p.lengths[b]) + p.offset;
-  n = n < 0 ? 0 : (n > p.T ? p.T : n);
+  n = (n > p.T ? p.T : n) - p.back;
+  n = n < 0 ? 0 : n;
   long long lo = 0;
   if (p.window >= 0) {
     lo = n - p.s - p.window;
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
   const int g = lane >> 2, t = lane & 3;
 
   // ------------------------------------------------ the block list: prefix per sequence, this CTA's run
-  const long long heads = static_cast<long long>(p.Hkv) * p.row_groups;
+  const long long heads = p.mult;  // (KV head, row group) items per sequence
   long long base = 0;
   for (int b0 = 0; b0 < p.B; b0 += kWarps * 32) {
     const int b = b0 + tid;
@@ -218,8 +219,8 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
     const int hr = static_cast<int>(rel / nb);  // (KV head, row group)
     const int j0 = static_cast<int>(rel - static_cast<long long>(hr) * nb);
     const int j1 = static_cast<int>(min(static_cast<long long>(nb), j0 + (end - pos)));
-    const int hk = hr / p.row_groups;
-    const int row0 = (hr - hk * p.row_groups) * R;
+    const int hk = hr / p.tiles;
+    const int row0 = (hr - hk * p.tiles) * R;
     const int rows = p.s * p.group;
 
     // ---------------------------------------------- query rows: B fragments and row factors
@@ -486,8 +487,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
       }
     __syncthreads();
     const bool whole = j0 == 0 && j1 == nb;
-    const long long item = b * heads + hr;
-    float* part = p.part + (blockIdx.x + item) * R * (D + 2);
+    float* part = p.part + (2LL * blockIdx.x + (j0 == 0)) * R * (D + 2);
     for (int w = tid; w < R * (D / 4); w += kWarps * 32) {
       const int r = w / (D / 4), c = (w - r * (D / 4)) * 4;
       if (row0 + r >= rows) continue;
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const uint2 y = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
         __nv_bfloat16* dst =
-            p.out + ((static_cast<long long>(b) * p.s + i) * p.H + hk * p.group + rr - i * p.group) * D + c;
+            p.out + b * p.o_sb + (static_cast<long long>(i) * p.H + hk * p.group + rr - i * p.group) * D + c;
         *reinterpret_cast<uint2*>(dst) = y;
       } else {
 #pragma unroll
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
 // One warp per output row: the partials of the CTAs whose runs met its item, in their order.
 // Rows of items inside one run were written already; rows without a visible block become zero.
 template <int D>
-__global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnParams p, int R) {
+__global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnParams p) {
   const int lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (b, token, head)
   if (row >= static_cast<long long>(p.B) * p.s * p.H) return;
@@ -537,12 +537,14 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
   const int b = static_cast<int>(bi / p.s);
   const int hk = h / p.group;
   const int rr = i * p.group + h - hk * p.group;
-  const int rg = rr / R, r = rr - rg * R;
-  const long long heads = static_cast<long long>(p.Hkv) * p.row_groups;
-  const long long run = p.plan[p.B + 1];
-  const long long nb = (p.plan[b + 1] - p.plan[b]) / heads;
-  const int hr = hk * p.row_groups + rg;
-  const long long from = p.plan[b] + hr * nb;
+  const int R = p.item_rows;
+  const int tile = rr / R, r = rr - tile * R;
+  const bool by_tile = p.entries_per_seq > 1 || p.mult == p.Hkv;  // (sequence, tile) entries of Hkv items
+  const long long entry = by_tile ? static_cast<long long>(b) * p.entries_per_seq + tile : b;
+  const int sub = by_tile ? hk : hk * p.tiles + tile;
+  const long long run = p.plan[static_cast<long long>(p.B) * p.entries_per_seq + 1];
+  const long long nb = (p.plan[entry + 1] - p.plan[entry]) / p.mult;
+  const long long from = p.plan[entry] + sub * nb;
   constexpr int N = D / 32;
   float a[N];
 #pragma unroll
@@ -551,16 +553,16 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
   if (nb > 0) {
     const long long c0 = from / run, c1 = (from + nb - 1) / run;
     if (c0 == c1) return;
-    const long long item = b * heads + hr;
-    const float* part = p.part + ((c0 + item) * R + r) * (D + 2);
     const long long step = static_cast<long long>(R) * (D + 2);
+    const float* part = p.part + r * (D + 2);
     const int n = static_cast<int>(c1 - c0 + 1);
-    for (int c = lane; c < n; c += 32) M = fmaxf(M, part[c * step + D]);
+    auto slot = [&](int c) { return part + (2 * (c0 + c) + (c == 0)) * step; };
+    for (int c = lane; c < n; c += 32) M = fmaxf(M, slot(c)[D]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
 #pragma unroll 4
     for (int c = 0; c < n; ++c) {
-      const float* x = part + c * step;
+      const float* x = slot(c);
       const float mw = x[D];
       const float f = M == -INFINITY ? 1.f : (mw == -INFINITY ? 0.f : exp2_fast(mw - M));
       L += x[D + 1] * f;
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  __nv_bfloat16* dst = p.out + row * D + lane * N;
+  __nv_bfloat16* dst = p.out + b * p.o_sb + (static_cast<long long>(i) * p.H + h) * D + lane * N;
 #pragma unroll
   for (int e = 0; e < N; e += 2)
     *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(a[e] * inv, a[e + 1] * inv);
@@ -590,43 +592,67 @@ int ctas_per_sm() {
   return cached;
 }
 
-int row_tiles(const CacheAttnParams& p) { return p.s * p.group <= 8 ? 1 : 2; }
+int row_groups_of_8(const CacheAttnParams& p) { return p.s * p.group <= 8 ? 1 : 2; }
 
 }  // namespace
 
-int cache_attn_max_seqs() { return kMaxSeqs; }
+bool cache_attn_many_rows(const CacheAttnParams& p) { return static_cast<long long>(p.s) * p.group > 16; }
+
+void cache_attn_limits(const CacheAttnParams& p, int* seqs, int* tokens) {
+  *seqs = kMaxSeqs;
+  *tokens = p.s;
+  if (cache_attn_many_rows(p)) {
+    // entries of one sequence: its row tiles; whole tokens, so that a launch's rows are a chunk again
+    const int most = kCacheTcEntries * kCacheTcRows / p.group;
+    *tokens = p.s < most ? p.s : (most < 1 ? 1 : most);
+    const int tiles = static_cast<int>((static_cast<long long>(*tokens) * p.group + kCacheTcRows - 1) / kCacheTcRows);
+    *seqs = kCacheTcEntries / tiles < 1 ? 1 : kCacheTcEntries / tiles;
+  }
+}
 
 void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long long* plan_words) {
-  const int rt = row_tiles(p), R = rt * 8;
-  p.row_groups = (p.s * p.group + R - 1) / R;
-  const int per_sm = D == 64 ? (rt == 1 ? ctas_per_sm<64, 1>() : ctas_per_sm<64, 2>())
-                             : (rt == 1 ? ctas_per_sm<128, 1>() : ctas_per_sm<128, 2>());
-  const long long items = static_cast<long long>(p.B) * p.Hkv * p.row_groups;
-  const long long most = items * ((p.T + kCacheBlock - 1) / kCacheBlock);  // key blocks if all caches were full
-  const long long want = (most + kMinRun - 1) / kMinRun;
-  const long long full = static_cast<long long>(device_sm_count()) * per_sm;
-  p.grid = static_cast<int>(want < 1 ? 1 : (want < full ? want : full));
-  *part_floats = (p.grid + items) * R * (D + 2);
-  *plan_words = p.B + 2;
+  const long long rows = static_cast<long long>(p.s) * p.group;
+  if (cache_attn_many_rows(p)) {
+    p.item_rows = kCacheTcRows;
+    p.tiles = static_cast<int>((rows + kCacheTcRows - 1) / kCacheTcRows);
+    p.entries_per_seq = p.tiles;
+    p.mult = p.Hkv;
+    p.grid = device_sm_count();
+  } else {
+    const int rt = row_groups_of_8(p);
+    p.item_rows = rt * 8;
+    p.tiles = static_cast<int>((rows + p.item_rows - 1) / p.item_rows);
+    p.entries_per_seq = 1;
+    p.mult = p.Hkv * p.tiles;
+    const int per_sm = D == 64 ? (rt == 1 ? ctas_per_sm<64, 1>() : ctas_per_sm<64, 2>())
+                               : (rt == 1 ? ctas_per_sm<128, 1>() : ctas_per_sm<128, 2>());
+    // key blocks if all caches were full
+    const long long most = static_cast<long long>(p.B) * p.mult * ((p.T + kCacheBlock - 1) / kCacheBlock);
+    const long long want = (most + kMinRun - 1) / kMinRun;
+    const long long full = static_cast<long long>(device_sm_count()) * per_sm;
+    p.grid = static_cast<int>(want < 1 ? 1 : (want < full ? want : full));
+  }
+  const long long entries = static_cast<long long>(p.B) * p.entries_per_seq;
+  *part_floats = 2LL * p.grid * p.item_rows * (D + 2);
+  *plan_words = entries + 2;
 }
 
 void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
-  const int rt = row_tiles(p);
+  const bool one = p.item_rows == 8;
+  if (cache_attn_many_rows(p))
+    cache_attn_tc(p, D, stream);
+  else if (D == 64)
+    one ? cache_attn_kernel<64, 1><<<p.grid, kWarps * 32, 0, stream>>>(p)
+        : cache_attn_kernel<64, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
+  else
+    one ? cache_attn_kernel<128, 1><<<p.grid, kWarps * 32, 0, stream>>>(p)
+        : cache_attn_kernel<128, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
   const long long rows = static_cast<long long>(p.B) * p.s * p.H;
   const unsigned merge = static_cast<unsigned>((rows + 3) / 4);
-  if (D == 64) {
-    if (rt == 1)
-      cache_attn_kernel<64, 1><<<p.grid, kWarps * 32, 0, stream>>>(p);
-    else
-      cache_attn_kernel<64, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
-    cache_attn_merge_kernel<64><<<merge, 128, 0, stream>>>(p, rt * 8);
-  } else {
-    if (rt == 1)
-      cache_attn_kernel<128, 1><<<p.grid, kWarps * 32, 0, stream>>>(p);
-    else
-      cache_attn_kernel<128, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
-    cache_attn_merge_kernel<128><<<merge, 128, 0, stream>>>(p, rt * 8);
-  }
+  if (D == 64)
+    cache_attn_merge_kernel<64><<<merge, 128, 0, stream>>>(p);
+  else
+    cache_attn_merge_kernel<128><<<merge, 128, 0, stream>>>(p);
 }
 
 }  // namespace pb

@@ -416,9 +416,10 @@ struct AppendParams {
 };
 void rotary_append(AppendParams p, int D, bool interleave, cudaStream_t stream);
 
-// Attention of s query tokens per sequence over the 8-bit caches (cache_attention.cu). Query i of
-// sequence b stands at position n - s + i with n = min(lengths[b] + offset, T) and sees the keys at
-// or before it, not more than `window` behind it (window >= 0).
+// Attention of s query tokens per sequence over the 8-bit caches (cache_attention.cu for few rows per
+// KV head, cache_attention_tc.cu for many). Query i of sequence b stands at position n - back - s + i
+// with n = min(lengths[b] + offset, T) and sees the keys at or before it, not more than `window` behind
+// it (window >= 0).
 struct CacheAttnParams {
   const __nv_bfloat16* q;  // [B, s, H, D], contiguous channels
   long long q_sb, q_ss, q_sh;
@@ -429,18 +430,31 @@ struct CacheAttnParams {
   const float* v_scale;
   long long ks_sb, ks_sh, vs_sb, vs_sh;
   const int* lengths;
-  __nv_bfloat16* out;      // [B, s, H, D] contiguous
-  int B, s, H, Hkv, T, group, offset, window;
+  __nv_bfloat16* out;      // [B, s, H, D], contiguous heads
+  long long o_sb;          // its stride per sequence
+  int B, s, H, Hkv, T, group, offset, back, window;
   float scale_log2;        // softmax scale * log2(e)
-  // workspace of the split form (sizes from cache_attn_plan)
-  float* part;             // [slots, rows, D + 2]
-  long long* plan;         // [B + 2] block prefix per sequence, total, blocks per CTA
-  int row_groups, grid;
+  // The work of a launch is one list of key blocks: per entry (a sequence, or a sequence's row tile)
+  // `mult` items of equal length, cut into equal runs over the CTAs. The piece of an item that a CTA border cuts goes
+  // to slot 2 CTA + 1 where the item begins in the CTA's run, to slot 2 CTA where it began before.
+  float* part;             // [slots, item_rows, D + 2]
+  long long* plan;         // [entries + 2]: first block of each entry, total, blocks per CTA
+  int item_rows;           // query rows per item
+  int tiles;               // row tiles per KV head: ceil(s * group / item_rows)
+  int entries_per_seq;     // 1, or `tiles`
+  int mult;                // Hkv * tiles, or Hkv
+  int grid;
   int* status;
 };
-// Rows (s * group) per work item, CTAs and workspace slots of the split form.
-int cache_attn_max_seqs();  // sequences per launch at most
+// Sequences (and tokens) that one launch takes at most, given what one of them needs.
+void cache_attn_limits(const CacheAttnParams& p, int* seqs, int* tokens);
+// Fills in the list's shape; the workspace sizes follow from it.
 void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long long* plan_words);
 void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream);
+// The two forms (cache_attn picks one by the rows per KV head).
+bool cache_attn_many_rows(const CacheAttnParams& p);
+void cache_attn_tc(const CacheAttnParams& p, int D, cudaStream_t stream);
+constexpr int kCacheTcEntries = 2048;  // entries of a launch's list (its prefix lies in shared memory)
+constexpr int kCacheTcRows = 256;
 
 }  // namespace pb

@@ -85,7 +85,11 @@ def test_attention_scale_sizes_and_large_scores(s: int) -> None:
     n = torch.tensor([t], dtype=torch.int32, device="cuda")
     base = ops.cache_attention(q, k, v, ks, vs, n).float()
     big = ops.cache_attention(q * 2.0**40, k, v, ks * 2.0**-30, vs * 2.0**20, n, scale=d**-0.5 * 2.0**-10).float()
-    assert torch.equal(big, base * 2.0**20)
+    # The many-row form adds log2 of V's scale to the exponents: the shift by 20 moves arguments of size up to 2**6
+    # by roundings of 2**-19 at most, the weights by 2**-18 of themselves and, numerator and sum, the output by
+    # 2**-17 max|V|; where that crosses a rounding border of bf16 the results are neighbours, 2**-7 apart at most.
+    limit = base.abs() * 2.0**-7 + 2.0**-17 * attention_tolerance(v, vs) * 2.0**8
+    assert ((big * 2.0**-20 - base).abs() <= limit).all()
     # one key outweighs all others: the output is its value row
     sharp = ops.cache_attention(q * 64, k, v, ks, vs, n)
     want = attend64(q * 64, k, v, ks, vs, [t])
