@@ -34,33 +34,16 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include "common.cuh"
-#include "kernels.h"
+#include "cache_attention_common.cuh"
 
 namespace pb {
 namespace {
 
+using namespace cache8;
+
 constexpr int kWarps = 4;
 constexpr int kMaxSeqs = 1024;  // sequences per launch (prefix table in shared memory)
 constexpr int kMinRun = 4;      // key blocks per CTA at least: one per warp
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two e4m3 bytes -> two halves (exact).
-__device__ __forceinline__ uint32_t f16x2_of(uint32_t two_bytes) {
-  uint32_t d;
-  asm("{\n.reg .b16 h;\ncvt.u16.u32 h, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(d) : "r"(two_bytes));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
@@ -77,34 +60,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Streaming 16-byte load (each cached byte is used once).
-__device__ __forceinline__ uint4 load16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
-
-// Bytes that hold an e4m3 NaN (0x7f, 0xff) as 0xff, others 0.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  const uint32_t m = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-  return (m >> 7) * 255u;
-}
-
-struct Item {
-  long long b;
-  int hk, rg;        // KV head, row group
-  long long n;       // keys in the cache, at most T
-  int first_block;   // first key block that any row of the sequence sees
-  int blocks;
-};
-
 // Keys of sequence b (0 .. T) and its visible key blocks.
 __device__ __forceinline__ int seq_blocks(const CacheAttnParams& p, int b, long long& n, int& first) {
-  n = static_cast<long long>(p.lengths[b]) + p.offset;
-  n = (n > p.T ? p.T : n) - p.back;
-  n = n < 0 ? 0 : n;
+  n = max(keys_of(p, b), 0LL);
   long long lo = 0;
   if (p.window >= 0) {
     lo = n - p.s - p.window;
@@ -192,13 +150,19 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
   __syncthreads();
   long long run = (total + gridDim.x - 1) / gridDim.x;
   run = run < kMinRun ? kMinRun : run;
-  if (blockIdx.x == 0) {
-    for (int b = tid; b <= p.B; b += kWarps * 32) p.plan[b] = prefix[b];
-    if (tid == 0) p.plan[p.B + 1] = run;
+  // sequences without a visible key: zeros
+  for (int e = blockIdx.x; e < p.B; e += gridDim.x) {
+    if (prefix[e + 1] != prefix[e]) continue;
+    uint4* dst = reinterpret_cast<uint4*>(p.out + e * p.o_sb);
+    for (int i = tid; i < p.s * p.H * (D / 8); i += kWarps * 32) dst[i] = make_uint4(0, 0, 0, 0);
   }
   long long pos = blockIdx.x * run;
   const long long end = min(pos + run, total);
-  if (pos >= end) return;
+  if (pos >= end) {
+    if (tid == 0) put_cut(p, blockIdx.x, {0, 0, 0, 0});
+    return;
+  }
+  Cut cut = {0, 0, 0, 0};
   int b = 0;
   {
     int hi = p.B;  // last sequence with prefix <= pos (empty ones share a prefix with their follower)
@@ -258,11 +222,8 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
       }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // 2^-k with amax in [2^k, 2^(k+1)); 1 for rows that are zero or not finite
-      const uint32_t ex = (__float_as_uint(amax) >> 23) & 255u;
-      const bool plain = ex < 2u || ex > 252u;
-      const float down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
-      const float up = plain ? 1.f : __uint_as_float(ex << 23);
+      float down, up;
+      row_power(amax, down, up);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         q[rt][ks][0] = pack_f16(x[4 * ks] * down, x[4 * ks + 1] * down);
@@ -487,6 +448,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
       }
     __syncthreads();
     const bool whole = j0 == 0 && j1 == nb;
+    if (j0 == 0 && j1 < nb) cut = {b, hk, row0, static_cast<int>((nb - j1 + run - 1) / run)};
     float* part = p.part + (2LL * blockIdx.x + (j0 == 0)) * R * (D + 2);
     for (int w = tid; w < R * (D / 4); w += kWarps * 32) {
       const int r = w / (D / 4), c = (w - r * (D / 4)) * 4;
@@ -522,49 +484,33 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
     __syncthreads();  // red is written again for the next item
     pos += j1 - j0;
   }
+  if (tid == 0) put_cut(p, blockIdx.x, cut);
 }
 
-// One warp per output row: the partials of the CTAs whose runs met its item, in their order.
-// Rows of items inside one run were written already; rows without a visible block become zero.
+// Merges the pieces of the item that CTA blockIdx.x of the main kernel began and did not finish: one
+// row at a time, the pieces spread over the four warps, each warp's in CTA order, the warps in order.
 template <int D>
 __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (b, token, head)
-  if (row >= static_cast<long long>(p.B) * p.s * p.H) return;
-  const int h = static_cast<int>(row % p.H);
-  const long long bi = row / p.H;
-  const int i = static_cast<int>(bi % p.s);
-  const int b = static_cast<int>(bi / p.s);
-  const int hk = h / p.group;
-  const int rr = i * p.group + h - hk * p.group;
-  const int R = p.item_rows;
-  const int tile = rr / R, r = rr - tile * R;
-  const bool by_tile = p.entries_per_seq > 1 || p.mult == p.Hkv;  // (sequence, tile) entries of Hkv items
-  const long long entry = by_tile ? static_cast<long long>(b) * p.entries_per_seq + tile : b;
-  const int sub = by_tile ? hk : hk * p.tiles + tile;
-  const long long run = p.plan[static_cast<long long>(p.B) * p.entries_per_seq + 1];
-  const long long nb = (p.plan[entry + 1] - p.plan[entry]) / p.mult;
-  const long long from = p.plan[entry] + sub * nb;
   constexpr int N = D / 32;
-  float a[N];
+  const Cut cut = get_cut(p, blockIdx.x);
+  if (cut.more == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float red[kWarps][D + 2];
+  const int rows = min(p.item_rows, p.s * p.group - cut.row0);
+  const long long step = static_cast<long long>(p.item_rows) * (D + 2);
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    const float* part = p.part + 2LL * blockIdx.x * step + r * (D + 2);
+    auto slot = [&](int c) { return part + (2 * c + (c == 0)) * step; };
+    float M = -INFINITY, L = 0.f, a[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) a[e] = 0.f;
-  float L = 0.f, M = -INFINITY;
-  if (nb > 0) {
-    const long long c0 = from / run, c1 = (from + nb - 1) / run;
-    if (c0 == c1) return;
-    const long long step = static_cast<long long>(R) * (D + 2);
-    const float* part = p.part + r * (D + 2);
-    const int n = static_cast<int>(c1 - c0 + 1);
-    auto slot = [&](int c) { return part + (2 * (c0 + c) + (c == 0)) * step; };
-    for (int c = lane; c < n; c += 32) M = fmaxf(M, slot(c)[D]);
+    for (int e = 0; e < N; ++e) a[e] = 0.f;
+    for (int c = warp + lane * kWarps; c <= cut.more; c += 32 * kWarps) M = fmaxf(M, slot(c)[D]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
 #pragma unroll 4
-    for (int c = 0; c < n; ++c) {
+    for (int c = warp; c <= cut.more; c += kWarps) {
       const float* x = slot(c);
-      const float mw = x[D];
-      const float f = M == -INFINITY ? 1.f : (mw == -INFINITY ? 0.f : exp2_fast(mw - M));
+      const float f = M == -INFINITY ? 1.f : exp2_fast(x[D] - M);
       L += x[D + 1] * f;
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
@@ -573,12 +519,30 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
         a[e + 1] = fmaf(y.y, f, a[e + 1]);
       }
     }
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  __nv_bfloat16* dst = p.out + b * p.o_sb + (static_cast<long long>(i) * p.H + h) * D + lane * N;
 #pragma unroll
-  for (int e = 0; e < N; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(a[e] * inv, a[e + 1] * inv);
+    for (int e = 0; e < N; ++e) red[warp][lane * N + e] = a[e];
+    if (lane == 0) {
+      red[warp][D] = M;
+      red[warp][D + 1] = L;
+    }
+    __syncthreads();
+    const int n = min(kWarps, cut.more + 1);  // warps that had a piece
+    if (threadIdx.x < D / 2) {
+      float mx = -INFINITY, l = 0.f, x0 = 0.f, x1 = 0.f;
+      for (int w = 0; w < n; ++w) mx = fmaxf(mx, red[w][D]);
+      for (int w = 0; w < n; ++w) {
+        const float f = mx == -INFINITY ? 1.f : exp2_fast(red[w][D] - mx);
+        l += red[w][D + 1] * f;
+        x0 = fmaf(red[w][2 * threadIdx.x], f, x0);
+        x1 = fmaf(red[w][2 * threadIdx.x + 1], f, x1);
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int rr = cut.row0 + r, i = rr / p.group, h = cut.hk * p.group + rr - i * p.group;
+      __nv_bfloat16* dst = p.out + cut.b * p.o_sb + (static_cast<long long>(i) * p.H + h) * D;
+      reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = pack_bf16x2(x0 * inv, x1 * inv);
+    }
+    __syncthreads();
+  }
 }
 
 template <int D, int RT>
@@ -632,9 +596,8 @@ void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long lon
     const long long full = static_cast<long long>(device_sm_count()) * per_sm;
     p.grid = static_cast<int>(want < 1 ? 1 : (want < full ? want : full));
   }
-  const long long entries = static_cast<long long>(p.B) * p.entries_per_seq;
   *part_floats = 2LL * p.grid * p.item_rows * (D + 2);
-  *plan_words = entries + 2;
+  *plan_words = 2LL * p.grid;
 }
 
 void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
@@ -647,8 +610,7 @@ void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
   else
     one ? cache_attn_kernel<128, 1><<<p.grid, kWarps * 32, 0, stream>>>(p)
         : cache_attn_kernel<128, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
-  const long long rows = static_cast<long long>(p.B) * p.s * p.H;
-  const unsigned merge = static_cast<unsigned>((rows + 3) / 4);
+  const dim3 merge(p.grid, p.item_rows < 32 ? p.item_rows : 32);
   if (D == 64)
     cache_attn_merge_kernel<64><<<merge, 128, 0, stream>>>(p);
   else

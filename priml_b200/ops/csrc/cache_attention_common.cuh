@@ -1,0 +1,76 @@
+// Pieces that the two forms of attention over an 8-bit cache share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace pb {
+namespace cache8 {
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two e4m3 bytes -> two halves (exact).
+__device__ __forceinline__ uint32_t f16x2_of(uint32_t two_bytes) {
+  uint32_t d;
+  asm("{\n.reg .b16 h;\ncvt.u16.u32 h, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(d) : "r"(two_bytes));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bytes of a cache row, past L1: a CTA reads each of them once.
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// 0xff in each byte of `w` that holds an e4m3 NaN (0x7f, 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  const uint32_t m = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return (m >> 7) * 255u;
+}
+
+// A query row whose largest magnitude is `amax` fits f16 after the exact factor `down`; `up` undoes it.
+// Rows that are zero, tiny or not finite stay as they are.
+__device__ __forceinline__ void row_power(float amax, float& down, float& up) {
+  const uint32_t ex = (__float_as_uint(amax) >> 23) & 255u;
+  const bool plain = ex < 2u || ex > 252u;
+  down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
+  up = plain ? 1.f : __uint_as_float(ex << 23);
+}
+
+// Keys of sequence b in the launch's view (what follows its last token taken off); may be negative.
+__device__ __forceinline__ long long keys_of(const CacheAttnParams& p, int b) {
+  const long long n = static_cast<long long>(p.lengths[b]) + p.offset;
+  return max((n > p.T ? p.T : n) - p.back, -(1LL << 30));
+}
+
+// The workspace's int64 words: [0, grid) hold per CTA the item that its run begins and leaves unfinished:
+// sequence, KV head, first row and the number of CTAs that hold its further pieces (0: none).
+struct Cut {
+  int b, hk, row0, more;
+};
+
+__device__ __forceinline__ void put_cut(const CacheAttnParams& p, int cta, const Cut& c) {
+  *reinterpret_cast<int4*>(p.plan + 2 * cta) = make_int4(c.b, c.hk, c.row0, c.more);
+}
+__device__ __forceinline__ Cut get_cut(const CacheAttnParams& p, int cta) {
+  const int4 v = *reinterpret_cast<const int4*>(p.plan + 2 * cta);
+  return {v.x, v.y, v.z, v.w};
+}
+
+}  // namespace cache8
+}  // namespace pb

@@ -8,52 +8,64 @@
 //
 // What bounds it: 4 D flops per (row, visible key) on the tensor cores, and one exp2 per pair on the
 // 16-per-clock special-function units: at D = 128 both take 2048 clocks per SM for 256 rows x 128 keys.
-// Feeding the MMA: kind::f16 needs both operands in 16 bits, so four warps convert each e4m3 tile to
-// f16 (exact, half an instruction per value) on its way from global to swizzled shared memory, once
-// per 256 rows. The block scales never touch the tiles: K's multiplies the scores of its 32 keys as
-// part of the exponent's multiply-add; V's goes into the weights, w = 2^(s + ev - M), M being the
-// running maximum of s + ev, so that w is within f16 whatever the scales, and the row sum adds
-// w 2^-ev. Queries are normalised by a power of two per row to fit f16.
+// Feeding the MMA: kind::f16 needs both operands in 16 bits, so the e4m3 tiles are converted to f16
+// (exact, half an instruction per value) on their way to swizzled shared memory, once per 256 rows.
+// The block scales never touch the tiles: K's multiplies the scores of its 32 keys as part of the
+// exponent's multiply-add; V's goes into the weights, w = 2^(s + ev - M), M being the running maximum
+// of s + ev, so that w is within f16 whatever the scales, and the row sum adds w 2^-ev. Queries are
+// normalised by a power of two per row to fit f16.
 //
-//   warps 0-3, 4-7  softmax of row tiles 0 and 1 (one row per thread); they also load their Q rows
-//   warps 8-11      K and V tiles: load 16 bytes a lane a tile ahead, convert, store swizzled
-//   warp 12         MMA issue: S_t = Q_t K^T, O_t += P_t V with P_t read from TMEM
-// While one group's softmax runs the tensor cores work for the other. Items of at most 128 rows use
-// both groups on the same rows: group t takes every other key tile, and the two results are merged.
-// TMEM: S_0 [0, 128) S_1 [128, 256) O_0 [256, 256 + D) O_1; P_t lies over S_t's first 64 columns.
-#include <cuda_fp16.h>
-
+//   warps 0-3, 4-7   softmax of row tiles 0 and 1 (one row per thread); they also load their Q rows
+//   warps 8-11       K tiles, e4m3 -> f16: 16-byte loads a tile ahead, held in registers
+//   warps 12-15      V tiles, the same, with the scales of both
+//   warps 16, 17     MMA issue for group t: S_t = Q_t K^T, O_t += P_t V with P_t read from TMEM
+//   warp 18          walks the run and hands its pieces out
+// The softmax goes 64 keys at a time with two score buffers per group: while it works on one, the
+// tensor cores fill the other and work for the other group. Items of at most 128 rows use both groups
+// on the same rows: group t takes half t of every key tile, and the two results are merged.
+// No role waits for the end of a piece but where it must: loads and conversions run ahead into the
+// next piece while the softmax warps finish the last.
+// TMEM: S_0 [0, 64) and [64, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1; P lies over the first half
+// of its scores.
 #include "attention_common.cuh"
+#include "cache_attention_common.cuh"
+
+#include <type_traits>
 
 namespace pb {
 namespace {
 
 using namespace attn;
+using namespace cache8;
 
 constexpr int kKeys = 128;  // keys per tile
-constexpr int kSoftmaxWarps = 8;
-constexpr int kConvertWarps = 4;
-constexpr int kThreads = 32 * (kSoftmaxWarps + kConvertWarps + 1);  // threads that work
-constexpr int kLaunch = 512;  // launched: whole warpgroups, so that the register split below is theirs
-// Registers per thread after the split; 512 threads are launched with 128 each (65,536).
-constexpr int kRegsSoftmax = 176, kRegsConvert = 96, kRegsMma = 56;
-static_assert(256 * kRegsSoftmax + 128 * kRegsConvert + 128 * kRegsMma <= kLaunch * 128, "register split");
-constexpr int kAllBarrier = 1;   // named barriers: every thread; the two softmax groups
-constexpr int kMergeBarrier = 2;
-constexpr float kShift = 7.f;    // weights are up to 2^(threshold + shift) = 2^15, within f16
+constexpr int kHalf = 64;   // keys per step of the softmax
+constexpr int kSoftmaxWarps = 8, kConvertWarps = 4;  // converting warps of K, and as many of V
+constexpr int kMmaWarp = kSoftmaxWarps + 2 * kConvertWarps, kWalkWarp = kMmaWarp + 2;
+constexpr int kLaunch = 640;  // whole warpgroups, so that the register split below is theirs
+// Registers per thread after the split; 640 threads are launched with 96 each.
+constexpr int kRegsSoftmax = 128, kRegsConvert = 72, kRegsIssue = 72;
+static_assert(256 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsIssue <= kLaunch * 96, "register split");
+constexpr int kGroupBarrier = 1;  // named barrier of the softmax warps
+constexpr float kShift = 7.f;     // weights are up to 2^(threshold + shift) = 2^15, within f16
+constexpr int kPolyOf4 = 1;       // of four pairs of weights this one takes exp2_poly
+constexpr int kPieces = 4;        // work pieces in flight between the walking warp and the others
+constexpr int kScratchCols = 32;  // columns that the groups exchange at a time
 
 template <int D>
 struct Cfg {
-  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kStages = 2;
   static constexpr int kQTile = (D / 64) * kChunkBytes;  // [128 rows][D] f16 in 64-column chunks
   static constexpr int kOffK = 2 * kQTile;
   static constexpr int kOffV = kOffK + kStages * kQTile;
-  static constexpr int kOffPrefix = kOffV + kStages * kQTile;
+  static constexpr int kScratchStride = kScratchCols + 4;  // floats
+  static constexpr int kScratch = 128 * kScratchStride * 4;
+  // The groups' exchange: query tile 1 is free in the pieces that need it.
+  static constexpr int kOffScratch = D == 128 ? kQTile : kOffV + kStages * kQTile;
+  static constexpr int kOffPrefix = kOffV + kStages * kQTile + (D == 128 ? 0 : kScratch);
   static constexpr int kOffBars = kOffPrefix + (kCacheTcEntries + 2) * 8;
   static constexpr int kBytes = kOffBars + 512 + 1024;
-  static constexpr int kMergeStride = D + 4;  // floats per row of the group merge (over the K and V stages)
-  static_assert(128 * kMergeStride * 4 <= 2 * kStages * kQTile, "the merge rows must fit the K and V stages");
-  static_assert(kBytes <= 227 * 1024, "shared memory");
+  static_assert(kBytes <= 227 * 1024 - 1024, "shared memory");
 };
 
 // Instruction descriptor: f16 A and B, fp32 accumulation.
@@ -62,52 +74,127 @@ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// TMEM loads together with their wait. The registers hold nothing before the wait, which the compiler
+// does not know: with the wait in a statement of its own it may move or spill them in between.
+__device__ __forceinline__ void tmem_read_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_read_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 
-__device__ __forceinline__ uint32_t f16x2_of(uint32_t two_bytes) {  // two e4m3 bytes, exact
-  uint32_t d;
-  asm("{\n.reg .b16 h;\ncvt.u16.u32 h, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(d) : "r"(two_bytes));
-  return d;
+__device__ __forceinline__ void tmem_read_x32x2(uint32_t taddr, uint32_t (&a)[32], uint32_t (&b)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
+      "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, "
+      "%53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),
+        "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(a[16]),
+        "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]), "=r"(a[24]),
+        "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]), "=r"(b[0]),
+        "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]),
+        "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15]), "=r"(b[16]), "=r"(b[17]),
+        "=r"(b[18]), "=r"(b[19]), "=r"(b[20]), "=r"(b[21]), "=r"(b[22]), "=r"(b[23]), "=r"(b[24]), "=r"(b[25]),
+        "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31])
+      : "r"(taddr), "r"(taddr + 32)
+      : "memory");
 }
 
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {  // 0xff where a byte is an e4m3 NaN
-  const uint32_t m = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-  return (m >> 7) * 255u;
+// 2^x of two values on the multiply-add pipes, for a part of the weights: the special-function units
+// bound the softmax. Range reduction to x = n + f, f in [0, 1), by adding 1.5 * 2^23 rounded down, and
+// a cubic with the least largest relative error on [0, 1) (7.5e-5, fitted here; f16 rounds by 2.4e-4).
+// Arguments below -126 give 2^-126, which f16 rounds to zero; NaN stays NaN.
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& e0, float& e1) {
+  float x0, x1;
+  f2_unpack(x2, x0, x1);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.f));
+  x2 = f2_pack(x0, x1);
+  const float magic = 12582912.f;
+  uint64_t n2, f2;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(n2) : "l"(x2), "l"(f2_pack(magic, magic)));
+  f2 = f2_sub(x2, f2_sub(n2, f2_pack(magic, magic)));
+  uint64_t y2 = f2_fma(f2, f2_pack(0.07802452f, 0.07802452f), f2_pack(0.22606724f, 0.22606724f));
+  y2 = f2_fma(y2, f2, f2_pack(0.69583347f, 0.69583347f));
+  y2 = f2_fma(y2, f2, f2_pack(0.99992523f, 0.99992523f));
+  float n0, n1;
+  f2_unpack(n2, n0, n1);  // the low bits hold n; a NaN stays in y2
+  y2 = f2_mul(y2, f2_pack(__uint_as_float((__float_as_uint(n0) << 23) + 0x3f800000u),
+                          __uint_as_float((__float_as_uint(n1) << 23) + 0x3f800000u)));
+  f2_unpack(y2, e0, e1);
 }
 
-__device__ __forceinline__ uint4 load16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+// Descriptors of 128-byte-swizzled tiles as their low words; all share the high word. The steps of a
+// product differ by constants in the low word, so one addition makes the next step's descriptor: the
+// issuing warp's few instructions per MMA are what the tensor cores wait for.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between 8-row groups
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr, uint32_t lbo_bytes) {
+  return (smem_addr >> 4) | ((lbo_bytes >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}" ::"r"(d),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
+      : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void bar_sync(int id) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+  return e != 0;
 }
+
+// A value that all lanes share, told to the compiler as such.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // Positions of a row tile's first and last rows, its visible key tiles and their count.
 struct Span {
-  int n;            // keys of the sequence in the launch's view (back already taken off)
-  int pos0, pos1;   // positions of the tile's first and last token
-  int first;        // first visible key tile
-  int count;        // visible key tiles
+  int n;           // keys of the sequence in the launch's view
+  int pos0, pos1;  // positions of the tile's first and last token
+  int first;       // first visible key tile
+  int count;       // visible key tiles
 };
 
 __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b, int r0, int nrows) {
   Span s;
-  long long n = static_cast<long long>(p.lengths[b]) + p.offset;
-  n = (n > p.T ? p.T : n) - p.back;
-  s.n = n < 0 ? 0 : static_cast<int>(n);
+  const int n = static_cast<int>(keys_of(p, b));
+  s.n = n < 0 ? 0 : n;
   // positions from the unclamped count: a sequence shorter than the chunk has queries before its start
-  const int base = static_cast<int>(n < -(1LL << 30) ? -(1LL << 30) : n) - p.s;
-  const int rows = p.s * p.group;
-  const int r1 = min(r0 + nrows, rows) - 1;
+  const int base = n - p.s;
+  const int r1 = min(r0 + nrows, p.s * p.group) - 1;
   s.pos0 = base + r0 / p.group;
   s.pos1 = base + r1 / p.group;
   const int lo = p.window >= 0 ? max(s.pos0 - p.window, 0) : 0;
@@ -116,21 +203,30 @@ __device__ __forceinline__ Span span_of(const CacheAttnParams& p, int b, int r0,
   return s;
 }
 
+// One piece of a CTA's run: key tiles [kt0, kt0 + count) of an item. Lies in shared memory.
 struct Piece {
-  int b, tile, hk;
-  Span sp;
-  int j0, j1;      // key tiles of the item in this CTA's run
-  bool both;       // at most 128 rows: the groups share them
+  int b, hk, row0;       // sequence, KV head, first row of the row tile
+  int n;                 // keys of the sequence
+  int base;              // position of the chunk's first token
+  int kt0, count;        // key tiles of this piece (count 0: the run is done)
+  int edge_hi, edge_lo;  // a key tile at k0 needs masks if k0 > edge_hi or k0 < edge_lo
+  int from[2], to[2];    // tiles of the piece that row tile 0 / 1 sees
+  int both;              // at most 128 rows: the groups share them and take half of each tile
+  int whole, begins;     // the piece is the whole item; it holds the item's first tile
 };
 
-// Walks a CTA's run of the list.
+// Walks a CTA's run of the list (one thread; its state lies in shared memory, not in registers).
 struct Walk {
-  const CacheAttnParams& p;
-  const long long* prefix;
-  long long pos, end;
+  long long pos, end, run;
   int entry;
-  __device__ Walk(const CacheAttnParams& p_, const long long* prefix_, long long pos_, long long end_)
-      : p(p_), prefix(prefix_), pos(pos_), end(end_), entry(0) {
+  Cut cut;
+  __device__ void start(const CacheAttnParams& p, const long long* prefix, long long pos_, long long end_,
+                        long long run_) {
+    pos = pos_;
+    end = end_;
+    run = run_;
+    entry = 0;
+    cut = {0, 0, 0, 0};
     int hi = p.B * p.entries_per_seq;
     while (hi - entry > 1) {
       const int mid = (entry + hi) >> 1;
@@ -138,19 +234,37 @@ struct Walk {
       else hi = mid;
     }
   }
-  __device__ bool next(Piece& x) {
-    if (pos >= end) return false;
+  __device__ void next(const CacheAttnParams& p, const long long* prefix, Piece& x) {
+    if (pos >= end) {
+      x.count = 0;
+      return;
+    }
     while (prefix[entry + 1] <= pos) ++entry;
-    x.b = entry / p.entries_per_seq;
-    x.tile = entry - x.b * p.entries_per_seq;
-    x.sp = span_of(p, x.b, x.tile * kCacheTcRows, kCacheTcRows);
+    const int b = entry / p.entries_per_seq, tile = entry - b * p.entries_per_seq;
+    const Span sp = span_of(p, b, tile * kCacheTcRows, kCacheTcRows);
     const long long rel = pos - prefix[entry];
-    x.hk = static_cast<int>(rel / x.sp.count);
-    x.j0 = static_cast<int>(rel - static_cast<long long>(x.hk) * x.sp.count);
-    x.j1 = static_cast<int>(min(static_cast<long long>(x.sp.count), x.j0 + (end - pos)));
-    x.both = p.s * p.group - x.tile * kCacheTcRows <= 128;
-    pos += x.j1 - x.j0;
-    return true;
+    const int hk = static_cast<int>(rel / sp.count);
+    const int j0 = static_cast<int>(rel - static_cast<long long>(hk) * sp.count);
+    const int j1 = static_cast<int>(min(static_cast<long long>(sp.count), j0 + (end - pos)));
+    x.b = b;
+    x.hk = hk;
+    x.row0 = tile * kCacheTcRows;
+    x.n = sp.n;
+    x.base = sp.pos0 - x.row0 / p.group;
+    x.kt0 = sp.first + j0;
+    x.count = j1 - j0;
+    x.edge_hi = sp.pos0 - kKeys + 1;
+    x.edge_lo = p.window >= 0 ? sp.pos1 - p.window : INT_MIN;
+    x.both = p.s * p.group - x.row0 <= 128;
+    x.whole = j0 == 0 && j1 == sp.count;
+    x.begins = j0 == 0;
+    for (int t = 0; t < 2; ++t) {
+      const Span st = span_of(p, b, x.row0 + 128 * t, 128);
+      x.from[t] = max(st.first - x.kt0, 0);
+      x.to[t] = st.count == 0 ? 0 : min(st.first + st.count - x.kt0, x.count);
+    }
+    if (j0 == 0 && j1 < sp.count) cut = {b, hk, x.row0, static_cast<int>((sp.count - j1 + run - 1) / run)};
+    pos += x.count;
   }
 };
 
@@ -165,37 +279,52 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
   uint8_t* sV = smem + C::kOffV;
   long long* prefix = reinterpret_cast<long long*>(smem + C::kOffPrefix);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
-  uint64_t* k_full = bars;             // [NS] four converting warps
-  uint64_t* k_empty = k_full + NS;     // [NS]
-  uint64_t* v_full = k_empty + NS;     // [NS]
-  uint64_t* v_empty = v_full + NS;     // [NS]
-  uint64_t* s_full = v_empty + NS;     // [2]
-  uint64_t* p_ready = s_full + 2;      // [2] four softmax warps
-  uint64_t* o_final = p_ready + 2;     // [2]
-  uint64_t* drain = o_final + 2;
+  uint64_t* k_full = bars;                      // [NS] four converting warps
+  uint64_t* k_empty = k_full + NS;              // [NS]
+  uint64_t* v_full = k_empty + NS;              // [NS]
+  uint64_t* v_empty = v_full + NS;              // [NS]
+  uint64_t* s_full = v_empty + NS;              // [2][2] group, score buffer
+  uint64_t* p_ready = s_full + 4;               // [2][2] four softmax warps
+  uint64_t* pv_done = p_ready + 4;              // [2]
+  uint64_t* o_final = pv_done + 2;              // [2]
+  uint64_t* q_full = o_final + 2;               // eight softmax warps
+  uint64_t* piece_full = q_full + 1;            // [kPieces]
+  uint64_t* piece_empty = piece_full + kPieces; // [kPieces] softmax, converting and MMA warps
+  uint64_t* drain = piece_empty + kPieces;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ long long warp_sum[kLaunch / 32];
   __shared__ uint32_t v_bad[NS][kConvertWarps][4];  // keys of an edge tile whose values hold a NaN
+  __shared__ alignas(16) float scales[NS][12];      // per 32 keys: K's scale, log2 of V's, its reciprocal
+  __shared__ Piece pieces[kPieces];
+  __shared__ Walk walk;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], kConvertWarps);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);  // both MMA warps
       mbar_init(&v_full[s], kConvertWarps);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_ready[t], 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[2 * t + i], 1);
+        mbar_init(&p_ready[2 * t + i], 4);
+      }
+      mbar_init(&pv_done[t], 1);
       mbar_init(&o_final[t], 1);
     }
-    mbar_init(drain, 1);
+    mbar_init(q_full, kSoftmaxWarps);
+    for (int s = 0; s < kPieces; ++s) {
+      mbar_init(&piece_full[s], 1);
+      mbar_init(&piece_empty[s], kSoftmaxWarps + 2 * kConvertWarps + 2);
+    }
+    mbar_init(drain, 2);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == kSoftmaxWarps + kConvertWarps) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -229,15 +358,19 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  long long run = (total + gridDim.x - 1) / gridDim.x;
-  run = run < 2 ? 2 : run;
-  if (blockIdx.x == 0) {
-    for (int e = tid; e <= entries; e += kLaunch) p.plan[e] = prefix[e];
-    if (tid == 0) p.plan[entries + 1] = run;
+  // row tiles without a visible key: zeros
+  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+    if (prefix[e + 1] != prefix[e]) continue;
+    const int b = e / p.entries_per_seq, r0 = (e - b * p.entries_per_seq) * kCacheTcRows;
+    const int rows = min(kCacheTcRows, p.s * p.group - r0);
+    for (int i = tid; i < rows * p.Hkv * (D / 8); i += kLaunch) {
+      const int c = i % (D / 8), hk = i / (D / 8) % p.Hkv, rr = r0 + i / (D / 8) / p.Hkv;
+      const int tok = rr / p.group;
+      __nv_bfloat16* dst =
+          p.out + b * p.o_sb + (static_cast<long long>(tok) * p.H + hk * p.group + rr - tok * p.group) * D + c * 8;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+    }
   }
-  const long long from = min(blockIdx.x * run, total);
-  Walk walk(p, prefix, from, min(from + run, total));
-  Piece x;
 
   if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------------ softmax + epilogue
@@ -247,123 +380,122 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + t * kKeys + lane_off;
     const uint32_t tO = tmem + 2 * kKeys + t * D + lane_off;
-    uint32_t tiles_before = 0, n_s = 0, n_seg = 0;
-    while (walk.next(x)) {
-      const int rows = p.s * p.group;
-      const int rr = x.tile * kCacheTcRows + (x.both ? r : t * 128 + r);  // row of the KV head
-      const bool row_ok = rr < rows;
+    uint32_t tiles_before = 0, n_seg = 0;
+    uint32_t s_phase = 0, n_pv = 0;  // parity of each score buffer's next fill; steps so far
+    bool ok = true;
+    for (; ok; ++n_seg) {
+      if (!(ok = mbar_wait_warp(&piece_full[n_seg % kPieces], (n_seg / kPieces) & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
+      const Piece& x = pieces[n_seg % kPieces];
+      const int count = x.count;
+      if (count == 0) break;
+      const bool both = x.both;
+      const int rr = x.row0 + (both ? r : t * 128 + r);  // row of the KV head
+      const bool row_ok = rr < p.s * p.group;
       const int tok = rr / p.group;
       const int head = x.hk * p.group + rr - tok * p.group;
       // ------------------------------ Q row: power of two, f16, swizzled tile
+      // (every MMA of the last piece is done: this thread saw o_final)
       float factor;
       {
         const __nv_bfloat16* src = p.q + x.b * p.q_sb + (row_ok ? tok * p.q_ss + head * p.q_sh : 0);
         float amax = 0.f;
-        if (row_ok) {
-#pragma unroll 4
+        uint4 raw[D / 8];
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          raw[c] = row_ok ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u[e] << 16)), fabsf(__uint_as_float(u[e] & 0xffff0000u))));
+        }
+        float down, up;
+        row_power(amax, down, up);
+        factor = up * fabsf(p.scale_log2);
+        if (p.scale_log2 < 0.f) down = -down;
+        if (!both || t == 0) {
+          uint8_t* tile = sQ + t * C::kQTile + r * 128;
+#pragma unroll
           for (int c = 0; c < D / 8; ++c) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(src + c * 8);
-            const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+            const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+            uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u[e] << 16)), fabsf(__uint_as_float(u[e] & 0xffff0000u))));
-          }
-        }
-        const uint32_t ex = (__float_as_uint(amax) >> 23) & 255u;
-        const bool plain = ex < 2u || ex > 252u;  // zero or not finite: as it is
-        float down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
-        factor = (plain ? 1.f : __uint_as_float(ex << 23)) * fabsf(p.scale_log2);
-        if (p.scale_log2 < 0.f) down = -down;
-        if (!x.both || t == 0) {
-          uint8_t* tile = sQ + t * C::kQTile + r * 128;
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            uint4 y = make_uint4(0, 0, 0, 0);
-            if (row_ok) {
-              const uint4 raw = *reinterpret_cast<const uint4*>(src + c * 8);
-              const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-              uint32_t h[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                h[e] = pack_f16(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
-              y = make_uint4(h[0], h[1], h[2], h[3]);
-            }
-            *reinterpret_cast<uint4*>(tile + (c >> 3) * kChunkBytes + (((c & 7) ^ (r & 7)) << 4)) = y;
+              h[e] = pack_f16(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
+            *reinterpret_cast<uint4*>(tile + (c >> 3) * kChunkBytes + (((c & 7) ^ (r & 7)) << 4)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
           }
         }
       }
       fence_proxy_async_smem();
-      bar_sync<kThreads>(kAllBarrier);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
 
       // ------------------------------ key tiles
-      const int pos = x.sp.pos0 - (x.tile * kCacheTcRows) / p.group + tok;
+      const int pos = x.base + tok;
       const int kmax = row_ok ? pos : -1;
       const int kmin = p.window >= 0 ? pos - p.window : 0;
-      const float* ksp = p.k_scale + x.b * p.ks_sb + x.hk * p.ks_sh;
-      const float* vsp = p.v_scale + x.b * p.vs_sb + x.hk * p.vs_sh;
-      const Span mine = x.both ? x.sp : span_of(p, x.b, x.tile * kCacheTcRows + t * 128, 128);
-      const int blocks = (x.sp.n + kCacheBlock - 1) / kCacheBlock;
+      const int edge_hi = x.edge_hi, edge_lo = x.edge_lo, kt0 = x.kt0;
+      // Step u of the group: 64 keys, half u & 1 of tile u / 2, or half t of tile u where the groups share the rows.
+      const int u_end = both ? count : 2 * x.to[t];
       float m = -INFINITY, l = 0.f;  // running maximum of s + ev (may lag by < 2^8), row sum of 2^(s - m + shift)
-      bool ok = true;
       int n = 0;
-      for (int j = x.j0; j < x.j1 && ok; ++j) {
-        const int kt = x.sp.first + j;
-        if (x.both ? ((j - x.j0) & 1) != t : (mine.count == 0 || kt < mine.first || kt >= mine.first + mine.count)) continue;
-        const int k0 = kt * kKeys;
-        float kc[4], ve[4], vi[4];  // score factor, exponent of V's scale and its reciprocal, per 32 keys
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int blk = k0 / kCacheBlock + i;
-          const float ks = blk < blocks ? ksp[blk] : 1.f, vs = blk < blocks ? vsp[blk] : 1.f;
-          kc[i] = fmaxf(factor * ks, 1e-37f);
-          ve[i] = __log2f(vs);
-          vi[i] = 1.f / vs;
-        }
-        if (!mbar_wait_warp_sleep(&s_full[t], n_s & 1, p.status, kTimeoutEpilogue, abort_flag)) { ok = false; break; }
+      for (int u = both ? 0 : 2 * x.from[t]; u < u_end; ++u) {
+        const int j = both ? u : u >> 1, half = both ? t : u & 1, buf = u & 1;
+        const int k0 = (kt0 + j) * kKeys;
+        const uint32_t tB = tS + buf * kHalf;
+        if (!(ok = mbar_wait_warp(&s_full[2 * t + buf], s_phase >> buf & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
+        s_phase ^= 1u << buf;
         tc_fence_after();
-        uint32_t v[kKeys];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
-        tmem_wait_ld();
-        const bool edge = k0 + kKeys - 1 > x.sp.pos0 || (p.window >= 0 && k0 < x.sp.pos1 - p.window);
-        if (edge) {
-          const uint32_t tile_no = tiles_before + (j - x.j0);
-          const int st = tile_no % NS;
-          if (!mbar_wait_warp(&v_full[st], (tile_no / NS) & 1, p.status, kTimeoutEpilogue, abort_flag)) { ok = false; break; }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+        // the tile's scales (and the flags below) come with its values
+        const uint32_t tile_no = tiles_before + j;
+        const int st = tile_no % NS;
+        if (!(ok = mbar_wait_warp(&v_full[st], (tile_no / NS) & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
+        const float2 ks2 = *reinterpret_cast<const float2*>(&scales[st][2 * half]);
+        const float2 ve2 = *reinterpret_cast<const float2*>(&scales[st][4 + 2 * half]);
+        const float2 vi2 = *reinterpret_cast<const float2*>(&scales[st][8 + 2 * half]);
+        const float kc[2] = {fmaxf(factor * ks2.x, 1e-37f), fmaxf(factor * ks2.y, 1e-37f)};
+        const float ve[2] = {ve2.x, ve2.y}, vi[2] = {vi2.x, vi2.y};
+        uint32_t va[32], vb[32];
+        tmem_read_x32x2(tB, va, vb);
+        if (k0 > edge_hi || k0 < edge_lo) {
+          auto mask = [&](uint32_t(&v)[32], int c) {  // scores of keys 32c .. 32c + 31 of the tile
             uint32_t bad = 0;
 #pragma unroll
             for (int w = 0; w < kConvertWarps; ++w) bad |= v_bad[st][w][c];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int key = k0 + 32 * c + i;
-              if (bad >> i & 1) v[32 * c + i] = 0x7fffffffu;
-              if (key > kmax || key < kmin) v[32 * c + i] = __float_as_uint(-INFINITY);
+              if (bad >> i & 1) v[i] = 0x7fffffffu;
+              if (key > kmax || key < kmin) v[i] = __float_as_uint(-INFINITY);
             }
-          }
+          };
+          mask(va, 2 * half);
+          mask(vb, 2 * half + 1);
         }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        auto top = [&](const uint32_t(&v)[32], int c) {
           float a = -INFINITY, a2 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            a = fmaxf(a, __uint_as_float(v[32 * c + i]));
-            a2 = fmaxf(a2, __uint_as_float(v[32 * c + i + 1]));
+            a = fmaxf(a, __uint_as_float(v[i]));
+            a2 = fmaxf(a2, __uint_as_float(v[i + 1]));
           }
-          mx = fmaxf(mx, fmaf(fmaxf(a, a2), kc[c], ve[c]));
-        }
+          return fmaf(fmaxf(a, a2), kc[c], ve[c]);
+        };
+        const float mx = fmaxf(top(va, 0), top(vb, 1));
         const bool grow = mx > m + kRescaleThreshold;
         const bool scale_o = grow && n > 0 && m != -INFINITY;
         if (__any_sync(0xffffffffu, scale_o)) {
+          // the last step's product must be in O; the one after it waits for this step's weights
+          if (!(ok = mbar_wait_warp(&pv_done[t], (n_pv - 1) & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
+          tc_fence_after();
           const float f = scale_o ? fast_exp2(m - mx) : 1.f;
           l *= f;
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
-            tmem_ld_32x32b_x16(tO + c * 16, o);
-            tmem_wait_ld();
+            tmem_read_x16(tO + c * 16, o);
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
             tmem_st_32x32b_x16(tO + c * 16, o);
@@ -371,18 +503,23 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         }
         if (grow) m = mx;
         const float ref = m == -INFINITY ? 0.f : kShift - m;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        auto weigh = [&](const uint32_t(&v)[32], int c) {
           const float add = ref + ve[c];
           const uint64_t mul2 = f2_pack(kc[c], kc[c]), add2 = f2_pack(add, add);
           uint64_t rs = f2_pack(0.f, 0.f);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[32 * c + 2 * i]), __uint_as_float(v[32 * c + 2 * i + 1])), mul2, add2),
-                      x0, x1);
-            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+            const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), mul2, add2);
+            float e0, e1;
+            if (i % 4 == kPolyOf4) {
+              exp2_poly(x2, e0, e1);
+            } else {
+              float x0, x1;
+              f2_unpack(x2, x0, x1);
+              e0 = fast_exp2(x0);
+              e1 = fast_exp2(x1);
+            }
             const uint64_t e2 = f2_pack(e0, e1);
             asm("add.rn.f32x2 %0, %0, %1;" : "+l"(rs) : "l"(e2));
             pk[i] = pack_f16(e0, e1);
@@ -390,280 +527,285 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           float r0, r1;
           f2_unpack(rs, r0, r1);
           l = fmaf(r0 + r1, vi[c], l);
-          tmem_st_32x32b_x16(tS + 16 * c, pk);
-        }
+          tmem_st_32x32b_x16(tB + 16 * c, pk);
+        };
+        weigh(va, 0);
+        weigh(vb, 1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[t]);
-        ++n_s;
+        if (lane == 0) mbar_arrive(&p_ready[2 * t + buf]);
+        ++n_pv;
         ++n;
       }
-      if (ok) ok = mbar_wait_warp_sleep(&o_final[t], n_seg & 1, p.status, kTimeoutEpilogue, abort_flag);
+      if (!ok || !(ok = mbar_wait_warp(&o_final[t], n_seg & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
       tc_fence_after();
 
       // ------------------------------ epilogue
-      const bool whole = x.j0 == 0 && x.j1 == x.sp.count;
-      float f_own = 1.f, f_other = 0.f;  // merge of the two groups' results (both == true)
-      float* scratch = reinterpret_cast<float*>(sK) + r * C::kMergeStride;
-      if (x.both) {
+      const bool whole = x.whole;
+      const bool write = row_ok && (!both || t == 0);
+      float f_own = 1.f, f_other = 0.f;  // merge of the two groups' results
+      float* scratch = reinterpret_cast<float*>(smem + C::kOffScratch) + r * C::kScratchStride;
+      if (both) {
         if (t == 1) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            if (ok && n > 0) {
-              tmem_ld_32x32b_x32(tO + c * 32, o);
-              tmem_wait_ld();
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(scratch + c * 32 + 4 * i) =
-                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-          scratch[D] = m;
-          scratch[D + 1] = l;
+          scratch[0] = m;
+          scratch[1] = l;
         }
-        bar_sync<kSoftmaxWarps * 32>(kMergeBarrier);
+        asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
         if (t == 0) {
-          const float m2 = scratch[D], l2 = scratch[D + 1];
+          const float m2 = scratch[0], l2 = scratch[1];
           const float mm = fmaxf(m, m2);
           f_own = m == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : fast_exp2(m - mm);
           f_other = m2 == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : fast_exp2(m2 - mm);
           l = l * f_own + l2 * f_other;
           m = mm;
         }
+        asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
       }
-      {
-        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        const bool write = row_ok && (!x.both || t == 0);
-        float* part = p.part + ((2LL * blockIdx.x + (x.j0 == 0)) * kCacheTcRows + (x.both ? r : t * 128 + r)) * (D + 2);
-        __nv_bfloat16* orow = p.out + x.b * p.o_sb + (static_cast<long long>(write ? tok : 0) * p.H + (write ? head : 0)) * D;
-        if (write && !whole) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
-        if (!x.both || t == 0) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float* part = p.part + ((2LL * blockIdx.x + x.begins) * kCacheTcRows + (both ? r : t * 128 + r)) * (D + 2);
+      __nv_bfloat16* orow = p.out + x.b * p.o_sb + (static_cast<long long>(write ? tok : 0) * p.H + (write ? head : 0)) * D;
+      if (write && !whole) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            if (ok && n > 0) {
-              tmem_ld_32x32b_x32(tO + c * 32, o);
-              tmem_wait_ld();
-            } else {
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_read_x32(tO + c * 32, o);
+        } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0u;
-            }
-            if (write) {
-              float y[32];
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        float y[32];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * f_own;
-              if (x.both) {
+        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(o[i]) * f_own;
+        if (both) {
+          if (t == 1) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = fmaf(scratch[c * 32 + i], f_other, y[i]);
-              }
-              if (whole) {
-                uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(scratch + 4 * i) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          }
+          asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
+          if (t == 0) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  dst[i] = make_uint4(pack_bf16x2(y[8 * i] * inv, y[8 * i + 1] * inv),
-                                      pack_bf16x2(y[8 * i + 2] * inv, y[8 * i + 3] * inv),
-                                      pack_bf16x2(y[8 * i + 4] * inv, y[8 * i + 5] * inv),
-                                      pack_bf16x2(y[8 * i + 6] * inv, y[8 * i + 7] * inv));
-              } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  *reinterpret_cast<float2*>(part + c * 32 + 2 * i) = make_float2(y[2 * i], y[2 * i + 1]);
-              }
+            for (int i = 0; i < 8; ++i) {
+              const float4 z = *reinterpret_cast<const float4*>(scratch + 4 * i);
+              y[4 * i] = fmaf(z.x, f_other, y[4 * i]);
+              y[4 * i + 1] = fmaf(z.y, f_other, y[4 * i + 1]);
+              y[4 * i + 2] = fmaf(z.z, f_other, y[4 * i + 2]);
+              y[4 * i + 3] = fmaf(z.w, f_other, y[4 * i + 3]);
             }
           }
+          asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
+        }
+        if (write && whole) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[i] = make_uint4(pack_bf16x2(y[8 * i] * inv, y[8 * i + 1] * inv),
+                                pack_bf16x2(y[8 * i + 2] * inv, y[8 * i + 3] * inv),
+                                pack_bf16x2(y[8 * i + 4] * inv, y[8 * i + 5] * inv),
+                                pack_bf16x2(y[8 * i + 6] * inv, y[8 * i + 7] * inv));
+        } else if (write) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) *reinterpret_cast<float2*>(part + c * 32 + 2 * i) = make_float2(y[2 * i], y[2 * i + 1]);
         }
       }
-      tiles_before += x.j1 - x.j0;
-      ++n_seg;
+      tiles_before += count;
       tc_fence_before();
-      bar_sync<kThreads>(kAllBarrier);
-      if (*abort_flag) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&piece_empty[n_seg % kPieces]);
     }
-  } else if (warp < kSoftmaxWarps + kConvertWarps) {
+  } else if (warp < kMmaWarp) {
     // ------------------------------------------------------------------ e4m3 -> f16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     constexpr int PR = D / 16;              // 16-byte pieces per row
-    constexpr int NP = kKeys * PR / 128;    // pieces per thread and tile
-    const int c = tid - kSoftmaxWarps * 32;
+    constexpr int NP = kKeys * PR / 128;    // pieces per thread and tile, in two batches
+    const bool is_v = warp >= kSoftmaxWarps + kConvertWarps;
+    const int c = (tid - kSoftmaxWarps * 32) & 127;
     const int piece = c % PR, row_c = c / PR;  // piece i: row row_c + i * (128 / PR)
+    uint8_t* tiles = is_v ? sV : sK;
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
     uint32_t tile_no = 0;
-    while (walk.next(x)) {
-      bar_sync<kThreads>(kAllBarrier);
-      const uint8_t* kp = p.k + x.b * p.k_sb + x.hk * p.k_sh + piece * 16;
-      const uint8_t* vp = p.v + x.b * p.v_sb + x.hk * p.v_sh + piece * 16;
-      uint4 kr[NP], vr[NP];
-      auto load = [&](uint4(&dst)[NP], const uint8_t* src, int k0) {
+    bool ok = true;
+    for (uint32_t seg = 0; ok; ++seg) {
+      if (!(ok = mbar_wait_warp(&piece_full[seg % kPieces], (seg / kPieces) & 1, p.status, kTimeoutProducer, abort_flag))) break;
+      const Piece& x = pieces[seg % kPieces];
+      const int count = x.count;
+      if (count == 0) break;
+      const int n_keys = x.n, edge_hi = x.edge_hi, edge_lo = x.edge_lo;
+      const uint8_t* src = (is_v ? p.v + x.b * p.v_sb + x.hk * p.v_sh : p.k + x.b * p.k_sb + x.hk * p.k_sh) + piece * 16;
+      // lanes 0-3 of the first V warp bring K's scales of the tile's blocks, lanes 4-7 V's
+      const bool brings = is_v && c < 8;
+      const float* scale = c < 4 ? p.k_scale + x.b * p.ks_sb + x.hk * p.ks_sh : p.v_scale + x.b * p.vs_sb + x.hk * p.vs_sh;
+      const int blocks = (n_keys + kCacheBlock - 1) / kCacheBlock;
+      auto scale_at = [&](int k0) {
+        const int blk = k0 / kCacheBlock + (c & 3);
+        return brings && blk < blocks ? scale[blk] : 1.f;
+      };
+      int k0 = x.kt0 * kKeys;
+      uint4 raw[NP];
+      auto load = [&](int from, int to, int base) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const int row = k0 + row_c + i * (128 / PR);
-          dst[i] = row < x.sp.n ? load16(src + static_cast<long long>(row) * D) : make_uint4(0, 0, 0, 0);
+          if (i < from || i >= to) continue;
+          const int row = base + row_c + i * (128 / PR);
+          raw[i] = row < n_keys ? load16(src + static_cast<long long>(row) * D) : make_uint4(0, 0, 0, 0);
         }
       };
-      auto store = [&](const uint4(&src)[NP], uint8_t* tile) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int row = row_c + i * (128 / PR);
-          uint8_t* base = tile + (piece >> 2) * kChunkBytes + row * 128;
-          const uint32_t u[4] = {src[i].x, src[i].y, src[i].z, src[i].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            h[2 * e] = f16x2_of(u[e]);
-            h[2 * e + 1] = f16x2_of(u[e] >> 16);
-          }
-          const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-          // the pieces of a row's two 64-channel chunks share banks: the upper chunk's lanes store
-          // their halves in the other order
-          const int p0 = 2 * (piece & 3);
-          const bool swap = piece >= 4;
-          *reinterpret_cast<uint4*>(base + (((p0 + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(base + (((p0 + !swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
-        }
-      };
-      int k0 = (x.sp.first + x.j0) * kKeys;
-      load(kr, kp, k0);
-      load(vr, vp, k0);
-      bool ok = true;
-      for (int j = x.j0; j < x.j1 && ok; ++j, ++tile_no, k0 += kKeys) {
+      load(0, NP, k0);
+      float sc = scale_at(k0);
+      for (int j = 0; j < count; ++j, ++tile_no, k0 += kKeys) {
         const int st = tile_no % NS;
-        const uint32_t ph = (tile_no / NS) & 1;
-        if (!mbar_wait_warp(&k_empty[st], ph ^ 1u, p.status, kTimeoutProducer, abort_flag)) { ok = false; break; }
-        store(kr, sK + st * C::kQTile);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[st]);
-        if (j + 1 < x.j1) load(kr, kp, k0 + kKeys);
-        if (!mbar_wait_warp(&v_empty[st], ph ^ 1u, p.status, kTimeoutProducer, abort_flag)) { ok = false; break; }
-        if (k0 + kKeys - 1 > x.sp.pos0 || (p.window >= 0 && k0 < x.sp.pos1 - p.window)) {
+        if (!(ok = mbar_wait_warp(&empty[st], ((tile_no / NS) & 1) ^ 1u, p.status, kTimeoutProducer, abort_flag))) break;
+        if (brings) {
+          scales[st][c] = c < 4 ? sc : __log2f(sc);
+          if (c >= 4) scales[st][4 + c] = 1.f / sc;
+          if (j + 1 < count) sc = scale_at(k0 + kKeys);
+        }
+        if (is_v && (k0 > edge_hi || k0 < edge_lo)) {
           // an edge tile: values that are NaN become zero, their keys are told to the softmax
           uint32_t bad[4] = {0, 0, 0, 0};
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            const uint32_t a = nan_bytes(vr[i].x), b2 = nan_bytes(vr[i].y), c2 = nan_bytes(vr[i].z), d2 = nan_bytes(vr[i].w);
-            vr[i] = make_uint4(vr[i].x & ~a, vr[i].y & ~b2, vr[i].z & ~c2, vr[i].w & ~d2);
+            const uint32_t a = nan_bytes(raw[i].x), b2 = nan_bytes(raw[i].y), c2 = nan_bytes(raw[i].z), d2 = nan_bytes(raw[i].w);
+            raw[i] = make_uint4(raw[i].x & ~a, raw[i].y & ~b2, raw[i].z & ~c2, raw[i].w & ~d2);
             const int row = row_c + i * (128 / PR);
             if (a | b2 | c2 | d2) bad[(i * (128 / PR)) >> 5] |= 1u << (row & 31);
           }
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const uint32_t all = __reduce_or_sync(0xffffffffu, bad[w]);
-            if (lane == 0) v_bad[st][warp - kSoftmaxWarps][w] = all;
+            if (lane == 0) v_bad[st][warp - kSoftmaxWarps - kConvertWarps][w] = all;
           }
         }
-        store(vr, sV + st * C::kQTile);
+        uint8_t* tile = tiles + st * C::kQTile;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int i = half * NP / 2; i < (half + 1) * NP / 2; ++i) {
+            const int row = row_c + i * (128 / PR);
+            uint8_t* base = tile + (piece >> 2) * kChunkBytes + row * 128;
+            const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            uint32_t f[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f[2 * e] = f16x2_of(u[e]);
+              f[2 * e + 1] = f16x2_of(u[e] >> 16);
+            }
+            const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+            // the pieces of a row's two 64-channel chunks share banks: the upper chunk's lanes store
+            // their halves in the other order
+            const int p0 = 2 * (piece & 3);
+            const bool swap = piece >= 4;
+            *reinterpret_cast<uint4*>(base + (((p0 + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
+            *reinterpret_cast<uint4*>(base + (((p0 + !swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
+          }
+          if (j + 1 < count) load(half * NP / 2, (half + 1) * NP / 2, k0 + kKeys);
+        }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[st]);
-        if (j + 1 < x.j1) load(vr, vp, k0 + kKeys);
+        if (lane == 0) mbar_arrive(&full[st]);
       }
-      bar_sync<kThreads>(kAllBarrier);
-      if (*abort_flag) break;
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&piece_empty[seg % kPieces]);
     }
   } else {
-    // ------------------------------------------------------------------ MMA issuer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-    if (warp > kSoftmaxWarps + kConvertWarps) return;  // fills the warpgroup
-    constexpr uint32_t idesc_s = idesc_f16(128, kKeys, false);
-    constexpr uint32_t idesc_o = idesc_f16(128, D, true);
-    uint32_t tile_no = 0, n_p[2] = {0, 0};
-    while (walk.next(x)) {
-      bar_sync<kThreads>(kAllBarrier);
-      tc_fence_after();
-      if (lane == 0) {
-        Span sp[2];
-        sp[0] = span_of(p, x.b, x.tile * kCacheTcRows, 128);
-        sp[1] = span_of(p, x.b, x.tile * kCacheTcRows + 128, 128);
-        const int jn = x.j1 - x.j0, kt0 = x.sp.first + x.j0;
-        int done[2] = {0, 0};
-        bool ok = true;
-        auto active = [&](int t, int j) {
-          return x.both || (sp[t].count > 0 && kt0 + j >= sp[t].first && kt0 + j < sp[t].first + sp[t].count);
-        };
-        auto issue_s = [&](int t, int j) -> bool {
-          const uint32_t no = tile_no + j, st = no % NS;
-          if (!mbar_wait(&k_full[st], (no / NS) & 1, p.status, kTimeoutMma, abort_flag)) return false;
-          tc_fence_after();
-          if (active(t, j)) {
-            const uint32_t q_base = smem_u32(sQ + (x.both ? 0 : t) * C::kQTile);
-            const uint32_t k_base = smem_u32(sK + st * C::kQTile);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == kWalkWarp && lane == 0) {
+      // ---------------------------------------------------------------- the run's pieces
+      const long long run = max((total + gridDim.x - 1) / gridDim.x, 2LL);
+      const long long from = min(blockIdx.x * run, total);
+      walk.start(p, prefix, from, min(from + run, total), run);
+      for (uint32_t seg = 0;; ++seg) {
+        Piece& x = pieces[seg % kPieces];
+        if (!mbar_wait(&piece_empty[seg % kPieces], ((seg / kPieces) & 1) ^ 1u, p.status, kTimeoutProducer, abort_flag)) break;
+        walk.next(p, prefix, x);
+        mbar_arrive(&piece_full[seg % kPieces]);
+        if (x.count == 0) break;
+      }
+      put_cut(p, blockIdx.x, walk.cut);
+    } else if (warp < kMmaWarp + 2) {
+      // ---------------------------------------------------------------- MMA issuers
+      // One warp per group: neither group's next product waits in program order for the other's weights.
+      // The whole warp walks along, so that its scalars stay in uniform registers.
+      constexpr uint32_t idesc_s = idesc_f16(128, kHalf, false);
+      constexpr uint32_t idesc_o = idesc_f16(128, D, true);
+      const bool leader = elect_one();
+      const uint32_t t = uniform(static_cast<uint32_t>(warp - kMmaWarp));
+      const uint32_t t_s = uniform(tmem) + t * kKeys, t_o = uniform(tmem) + 2 * kKeys + t * D;
+      const uint32_t q0_low = uniform(desc_low(smem_u32(sQ), 16));
+      const uint32_t k0_low = uniform(desc_low(smem_u32(sK), 16)), v0_low = uniform(desc_low(smem_u32(sV), kChunkBytes));
+      uint32_t tile_no = 0, p_phase = 0;
+      bool ok = true;
+      for (uint32_t seg = 0; ok; ++seg) {
+        if (!(ok = mbar_wait_warp(&piece_full[seg % kPieces], (seg / kPieces) & 1, p.status, kTimeoutMma, abort_flag))) break;
+        const Piece& x = pieces[seg % kPieces];
+        const int jn = uniform(x.count);
+        if (jn == 0) break;
+        if (!(ok = mbar_wait_warp(q_full, seg & 1, p.status, kTimeoutMma, abort_flag))) break;
+        tc_fence_after();
+        const bool both = uniform(x.both);
+        const int steps = both ? jn : 2 * jn;
+        const int from = both ? 0 : 2 * uniform(x.from[t]), to = both ? jn : 2 * uniform(x.to[t]);
+        __syncwarp();
+        if (leader) mbar_arrive(&piece_empty[seg % kPieces]);
+        const uint32_t q_low = q0_low + (both ? 0 : t * (C::kQTile / 16));
+        uint32_t more = 0;  // whether O_t holds products of this piece
+        for (int u = -2; u < steps; ++u) {
+          if (u >= 0) {  // O_t += P_t V of step u
+            const uint32_t no = tile_no + (both ? u : u >> 1), st = no % NS, half = both ? t : u & 1, buf = u & 1;
+            // A group that does not see the tile waits for it all the same: releasing tiles ahead of their
+            // being filled, it would stand in for the other group's release.
+            if (!(ok = mbar_wait_warp(&v_full[st], (no / NS) & 1, p.status, kTimeoutMma, abort_flag))) break;
+            if (u >= from && u < to) {
+              if (!(ok = mbar_wait_warp(&p_ready[2 * t + buf], p_phase >> buf & 1, p.status, kTimeoutMma, abort_flag))) break;
+              p_phase ^= 1u << buf;
+              tc_fence_after();
+              const uint32_t v_low = v0_low + (st * C::kQTile + half * (kHalf * 128)) / 16, pw = t_s + buf * kHalf;
+              if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              umma_f16(tmem + t * kKeys, kmajor_desc(q_base, kk), kmajor_desc(k_base, kk), idesc_s, kk > 0);
-            umma_commit(&s_full[t]);
+                for (int kk = 0; kk < kHalf / 16; ++kk)
+                  mma_ts(t_o, pw + kk * 8, v_low + kk * (2048 / 16), idesc_o, kk > 0 ? 1 : more);
+                umma_commit(&pv_done[t]);
+              }
+              more = 1;
+            }
+            if ((both || half == 1) && leader) umma_commit(&v_empty[st]);
           }
-          return true;
-        };
-        auto issue_pv = [&](int t, int j) -> bool {
-          if (!active(t, j)) return true;
-          const uint32_t no = tile_no + j, st = no % NS;
-          if (!mbar_wait(&p_ready[t], n_p[t] & 1, p.status, kTimeoutMma, abort_flag)) return false;
-          if (!mbar_wait(&v_full[st], (no / NS) & 1, p.status, kTimeoutMma, abort_flag)) return false;
-          tc_fence_after();
-          const uint32_t v_base = smem_u32(sV + st * C::kQTile);
+          if (u + 2 < steps) {  // S_t of the step after the next, into the buffer that step u left
+            const uint32_t w = u + 2, no = tile_no + (both ? w : w >> 1), st = no % NS, half = both ? t : w & 1, buf = w & 1;
+            if (!(ok = mbar_wait_warp(&k_full[st], (no / NS) & 1, p.status, kTimeoutMma, abort_flag))) break;
+            if (static_cast<int>(w) >= from && static_cast<int>(w) < to) {
+              tc_fence_after();
+              const uint32_t k_low = k0_low + (st * C::kQTile + half * (kHalf * 128)) / 16, d = t_s + buf * kHalf;
+              if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            umma_f16_tmem_a(tmem + 2 * kKeys + t * D, tmem + t * kKeys + kk * 8, mnmajor_desc(v_base, kk), idesc_o,
-                            (done[t] | kk) != 0);
-          ++n_p[t];
-          ++done[t];
-          return true;
-        };
-        auto k_done = [&](int j) { umma_commit(&k_empty[(tile_no + j) % NS]); };
-        auto v_done = [&](int j) { umma_commit(&v_empty[(tile_no + j) % NS]); };
-        if (x.both) {
-          // one row tile: group t works on key tiles t, t + 2, ...
-          ok = issue_s(0, 0);
-          if (ok) k_done(0);
-          if (ok && jn > 1) {
-            ok = issue_s(1, 1);
-            if (ok) k_done(1);
-          }
-          for (int j = 0; j < jn && ok; ++j) {
-            const int t = j & 1;
-            if (!(ok = issue_pv(t, j))) break;
-            v_done(j);
-            if (j + 2 < jn) {
-              if (!(ok = issue_s(t, j + 2))) break;
-              k_done(j + 2);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const uint32_t step = ((kk >> 2) * kChunkBytes + (kk & 3) * 32) / 16;
+                  mma_ss(d, q_low + step, k_low + step, idesc_s, kk > 0);
+                }
+                umma_commit(&s_full[2 * t + buf]);
+              }
             }
-          }
-        } else {
-          ok = issue_s(0, 0) && issue_s(1, 0);
-          if (ok) k_done(0);
-          for (int j = 0; j < jn && ok; ++j) {
-            if (!(ok = issue_pv(0, j))) break;
-            if (j + 1 < jn && !(ok = issue_s(0, j + 1))) break;
-            if (!(ok = issue_pv(1, j))) break;
-            v_done(j);
-            if (j + 1 < jn) {
-              if (!(ok = issue_s(1, j + 1))) break;
-              k_done(j + 1);
-            }
+            if ((both || half == 1) && leader) umma_commit(&k_empty[st]);
           }
         }
-        umma_commit(&o_final[0]);
-        umma_commit(&o_final[1]);
+        if (leader) umma_commit(&o_final[t]);
         tile_no += jn;
       }
-      __syncwarp();
-      bar_sync<kThreads>(kAllBarrier);
-      if (*abort_flag) break;
-    }
-    if (lane == 0) {
-      umma_commit(drain);
-      mbar_wait(drain, 0, p.status, kTimeoutDrain, nullptr);
+      if (leader) {
+        umma_commit(drain);
+        mbar_wait(drain, 0, p.status, kTimeoutDrain, nullptr);
+      }
     }
     __syncwarp();
   }
   tc_fence_before();
-  bar_sync<kThreads>(kAllBarrier);
+  __syncthreads();
   tc_fence_after();
-  if (warp == kSoftmaxWarps + kConvertWarps) {
+  if (warp == kMmaWarp) {
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }

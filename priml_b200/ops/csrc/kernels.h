@@ -435,10 +435,11 @@ struct CacheAttnParams {
   int B, s, H, Hkv, T, group, offset, back, window;
   float scale_log2;        // softmax scale * log2(e)
   // The work of a launch is one list of key blocks: per entry (a sequence, or a sequence's row tile)
-  // `mult` items of equal length, cut into equal runs over the CTAs. The piece of an item that a CTA border cuts goes
-  // to slot 2 CTA + 1 where the item begins in the CTA's run, to slot 2 CTA where it began before.
-  float* part;             // [slots, item_rows, D + 2]
-  long long* plan;         // [entries + 2]: first block of each entry, total, blocks per CTA
+  // `mult` items of equal length, cut into equal runs over the CTAs. The piece of an item that a CTA
+  // border cuts goes to slot 2 CTA + 1 where the item begins in the CTA's run, to slot 2 CTA where it
+  // began before.
+  float* part;             // [2 grid, item_rows, D + 2]: unnormalised output, maximum, sum
+  long long* plan;         // [2 grid]: the cut items, 16 bytes per CTA
   int item_rows;           // query rows per item
   int tiles;               // row tiles per KV head: ceil(s * group / item_rows)
   int entries_per_seq;     // 1, or `tiles`
@@ -446,7 +447,7 @@ struct CacheAttnParams {
   int grid;
   int* status;
 };
-// Sequences (and tokens) that one launch takes at most, given what one of them needs.
+// Sequences (and tokens) that one launch takes at most.
 void cache_attn_limits(const CacheAttnParams& p, int* seqs, int* tokens);
 // Fills in the list's shape; the workspace sizes follow from it.
 void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long long* plan_words);
@@ -454,7 +455,7 @@ void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream);
 // The two forms (cache_attn picks one by the rows per KV head).
 bool cache_attn_many_rows(const CacheAttnParams& p);
 void cache_attn_tc(const CacheAttnParams& p, int D, cudaStream_t stream);
-constexpr int kCacheTcEntries = 2048;  // entries of a launch's list (its prefix lies in shared memory)
+constexpr int kCacheTcEntries = 1024;  // entries of a launch's list (its prefix lies in shared memory)
 constexpr int kCacheTcRows = 256;
 
 }  // namespace pb
