@@ -43,7 +43,8 @@ using namespace cache8;
 
 constexpr int kWarps = 4;
 constexpr int kMaxSeqs = 1024;  // sequences per launch (prefix table in shared memory)
-constexpr int kMinRun = 4;      // key blocks per CTA at least: one per warp
+constexpr int kItemCost = 4;    // an item's start and end cost a CTA about as much as this many key blocks
+constexpr int kMinRun = kItemCost + 4;  // list entries per CTA at least: an item's cost and a block per warp
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
@@ -114,7 +115,7 @@ __device__ __forceinline__ void load_v(Step<D, RT>& st, const uint8_t* v, int ba
 }
 
 template <int D, int RT>
-__global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kernel(const CacheAttnParams p) {
   constexpr int R = RT * 8;         // query rows per item
   constexpr int KS = D / 16;        // k-steps of the score product = m-tiles of the value product
   __shared__ long long prefix[kMaxSeqs + 1];
@@ -130,7 +131,11 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
     const int b = b0 + tid;
     long long n;
     int first;
-    long long x = b < p.B ? seq_blocks(p, b, n, first) * heads : 0;
+    long long x = 0;
+    if (b < p.B) {
+      const int blocks = seq_blocks(p, b, n, first);
+      x = blocks > 0 ? (blocks + kItemCost) * heads : 0;
+    }
     const long long own = x;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -180,9 +185,13 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
     const int nb = seq_blocks(p, b, n64, first);
     const int n = static_cast<int>(n64);
     const long long rel = pos - prefix[b];
-    const int hr = static_cast<int>(rel / nb);  // (KV head, row group)
-    const int j0 = static_cast<int>(rel - static_cast<long long>(hr) * nb);
-    const int j1 = static_cast<int>(min(static_cast<long long>(nb), j0 + (end - pos)));
+    const int len = nb + kItemCost;             // the item's length in the list: its cost, then its blocks
+    const int hr = static_cast<int>(rel / len);  // (KV head, row group)
+    const int v0 = static_cast<int>(rel - static_cast<long long>(hr) * len);
+    const int v1 = static_cast<int>(min(static_cast<long long>(len), v0 + (end - pos)));
+    const int j0 = max(v0 - kItemCost, 0), j1 = max(v1 - kItemCost, 0);
+    pos += v1 - v0;
+    if (j1 == j0) continue;  // the run ends inside the cost: the blocks are all the next CTA's
     const int hk = hr / p.tiles;
     const int row0 = (hr - hk * p.tiles) * R;
     const int rows = p.s * p.group;
@@ -482,33 +491,45 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const CacheAttn
       }
     }
     __syncthreads();  // red is written again for the next item
-    pos += j1 - j0;
   }
   if (tid == 0) put_cut(p, blockIdx.x, cut);
 }
 
-// Merges the pieces of the item that CTA blockIdx.x of the main kernel began and did not finish: one
-// row at a time, the pieces spread over the four warps, each warp's in CTA order, the warps in order.
+// Merges the pieces of the item that CTA blockIdx.x of the main kernel began and did not finish. Few
+// pieces: a warp per row. Many (one long sequence spread over the grid): a CTA per row, its warps
+// taking every eighth piece. Either way the order of the sums is fixed by the pieces' order.
+constexpr int kMergeWarps = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnParams p) {
+__device__ __forceinline__ void store_row(const CacheAttnParams& p, const Cut& cut, int r, int c, float x0, float x1) {
+  const int rr = cut.row0 + r, i = rr / p.group, h = cut.hk * p.group + rr - i * p.group;
+  __nv_bfloat16* dst = p.out + cut.b * p.o_sb + (static_cast<long long>(i) * p.H + h) * D + c;
+  *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(x0, x1);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) cache_attn_merge_kernel(const CacheAttnParams p) {
   constexpr int N = D / 32;
   const Cut cut = get_cut(p, blockIdx.x);
   if (cut.more == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ float red[kWarps][D + 2];
+  __shared__ float red[kMergeWarps][D + 2];
   const int rows = min(p.item_rows, p.s * p.group - cut.row0);
   const long long step = static_cast<long long>(p.item_rows) * (D + 2);
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+  const bool few = cut.more < kMergeWarps;
+  const int first = few ? 0 : warp, by = few ? 1 : kMergeWarps;  // this warp's pieces
+  const int r0 = few ? blockIdx.y * kMergeWarps + warp : blockIdx.y, r_step = few ? gridDim.y * kMergeWarps : gridDim.y;
+  for (int r = r0; r < rows; r += r_step) {
     const float* part = p.part + 2LL * blockIdx.x * step + r * (D + 2);
     auto slot = [&](int c) { return part + (2 * c + (c == 0)) * step; };
     float M = -INFINITY, L = 0.f, a[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) a[e] = 0.f;
-    for (int c = warp + lane * kWarps; c <= cut.more; c += 32 * kWarps) M = fmaxf(M, slot(c)[D]);
+    for (int c = first + lane * by; c <= cut.more; c += 32 * by) M = fmaxf(M, slot(c)[D]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-#pragma unroll 4
-    for (int c = warp; c <= cut.more; c += kWarps) {
+#pragma unroll 8
+    for (int c = first; c <= cut.more; c += by) {
       const float* x = slot(c);
       const float f = M == -INFINITY ? 1.f : exp2_fast(x[D] - M);
       L += x[D + 1] * f;
@@ -519,6 +540,12 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
         a[e + 1] = fmaf(y.y, f, a[e + 1]);
       }
     }
+    if (few) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+      for (int e = 0; e < N; e += 2) store_row<D>(p, cut, r, lane * N + e, a[e] * inv, a[e + 1] * inv);
+      continue;
+    }
 #pragma unroll
     for (int e = 0; e < N; ++e) red[warp][lane * N + e] = a[e];
     if (lane == 0) {
@@ -526,20 +553,19 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
       red[warp][D + 1] = L;
     }
     __syncthreads();
-    const int n = min(kWarps, cut.more + 1);  // warps that had a piece
     if (threadIdx.x < D / 2) {
       float mx = -INFINITY, l = 0.f, x0 = 0.f, x1 = 0.f;
-      for (int w = 0; w < n; ++w) mx = fmaxf(mx, red[w][D]);
-      for (int w = 0; w < n; ++w) {
+#pragma unroll
+      for (int w = 0; w < kMergeWarps; ++w) mx = fmaxf(mx, red[w][D]);
+#pragma unroll
+      for (int w = 0; w < kMergeWarps; ++w) {
         const float f = mx == -INFINITY ? 1.f : exp2_fast(red[w][D] - mx);
         l += red[w][D + 1] * f;
         x0 = fmaf(red[w][2 * threadIdx.x], f, x0);
         x1 = fmaf(red[w][2 * threadIdx.x + 1], f, x1);
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int rr = cut.row0 + r, i = rr / p.group, h = cut.hk * p.group + rr - i * p.group;
-      __nv_bfloat16* dst = p.out + cut.b * p.o_sb + (static_cast<long long>(i) * p.H + h) * D;
-      reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = pack_bf16x2(x0 * inv, x1 * inv);
+      store_row<D>(p, cut, r, 2 * threadIdx.x, x0 * inv, x1 * inv);
     }
     __syncthreads();
   }
@@ -591,7 +617,7 @@ void cache_attn_plan(CacheAttnParams& p, int D, long long* part_floats, long lon
     const int per_sm = D == 64 ? (rt == 1 ? ctas_per_sm<64, 1>() : ctas_per_sm<64, 2>())
                                : (rt == 1 ? ctas_per_sm<128, 1>() : ctas_per_sm<128, 2>());
     // key blocks if all caches were full
-    const long long most = static_cast<long long>(p.B) * p.mult * ((p.T + kCacheBlock - 1) / kCacheBlock);
+    const long long most = static_cast<long long>(p.B) * p.mult * ((p.T + kCacheBlock - 1) / kCacheBlock + kItemCost);
     const long long want = (most + kMinRun - 1) / kMinRun;
     const long long full = static_cast<long long>(device_sm_count()) * per_sm;
     p.grid = static_cast<int>(want < 1 ? 1 : (want < full ? want : full));
@@ -612,9 +638,9 @@ void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
         : cache_attn_kernel<128, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
   const dim3 merge(p.grid, p.item_rows < 32 ? p.item_rows : 32);
   if (D == 64)
-    cache_attn_merge_kernel<64><<<merge, 128, 0, stream>>>(p);
+    cache_attn_merge_kernel<64><<<merge, kMergeWarps * 32, 0, stream>>>(p);
   else
-    cache_attn_merge_kernel<128><<<merge, 128, 0, stream>>>(p);
+    cache_attn_merge_kernel<128><<<merge, kMergeWarps * 32, 0, stream>>>(p);
 }
 
 }  // namespace pb

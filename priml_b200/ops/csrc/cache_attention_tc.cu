@@ -44,10 +44,12 @@ constexpr int kSoftmaxWarps = 8, kConvertWarps = 4;  // converting warps of K, a
 constexpr int kMmaWarp = kSoftmaxWarps + 2 * kConvertWarps, kWalkWarp = kMmaWarp + 2;
 constexpr int kLaunch = 640;  // whole warpgroups, so that the register split below is theirs
 // Registers per thread after the split; 640 threads are launched with 96 each.
-constexpr int kRegsSoftmax = 128, kRegsConvert = 72, kRegsIssue = 72;
+constexpr int kRegsSoftmax = 136, kRegsConvert = 72, kRegsIssue = 64;
 static_assert(256 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsIssue <= kLaunch * 96, "register split");
 constexpr int kGroupBarrier = 1;  // named barrier of the softmax warps
 constexpr float kShift = 7.f;     // weights are up to 2^(threshold + shift) = 2^15, within f16
+constexpr int kItemCost = 3;       // an item's start and end cost a CTA about as much as this many key tiles
+constexpr int kAhead = 6;          // key tiles that are asked for in L2 before their loads
 constexpr int kPolyOf4 = 1;       // of four pairs of weights this one takes exp2_poly
 constexpr int kPieces = 4;        // work pieces in flight between the walking warp and the others
 constexpr int kScratchCols = 32;  // columns that the groups exchange at a time
@@ -235,17 +237,26 @@ struct Walk {
     }
   }
   __device__ void next(const CacheAttnParams& p, const long long* prefix, Piece& x) {
-    if (pos >= end) {
-      x.count = 0;
-      return;
-    }
-    while (prefix[entry + 1] <= pos) ++entry;
-    const int b = entry / p.entries_per_seq, tile = entry - b * p.entries_per_seq;
-    const Span sp = span_of(p, b, tile * kCacheTcRows, kCacheTcRows);
-    const long long rel = pos - prefix[entry];
-    const int hk = static_cast<int>(rel / sp.count);
-    const int j0 = static_cast<int>(rel - static_cast<long long>(hk) * sp.count);
-    const int j1 = static_cast<int>(min(static_cast<long long>(sp.count), j0 + (end - pos)));
+    int b, tile, hk, j0, j1;
+    Span sp;
+    do {
+      if (pos >= end) {
+        x.count = 0;
+        return;
+      }
+      while (prefix[entry + 1] <= pos) ++entry;
+      b = entry / p.entries_per_seq;
+      tile = entry - b * p.entries_per_seq;
+      sp = span_of(p, b, tile * kCacheTcRows, kCacheTcRows);
+      const long long rel = pos - prefix[entry];
+      const int len = sp.count + kItemCost;  // the item's length in the list: its cost, then its tiles
+      hk = static_cast<int>(rel / len);
+      const int v0 = static_cast<int>(rel - static_cast<long long>(hk) * len);
+      const int v1 = static_cast<int>(min(static_cast<long long>(len), v0 + (end - pos)));
+      j0 = max(v0 - kItemCost, 0);
+      j1 = max(v1 - kItemCost, 0);
+      pos += v1 - v0;
+    } while (j1 == j0);  // the run ends inside the cost: the tiles are all the next CTA's
     x.b = b;
     x.hk = hk;
     x.row0 = tile * kCacheTcRows;
@@ -264,7 +275,6 @@ struct Walk {
       x.to[t] = st.count == 0 ? 0 : min(st.first + st.count - x.kt0, x.count);
     }
     if (j0 == 0 && j1 < sp.count) cut = {b, hk, x.row0, static_cast<int>((sp.count - j1 + run - 1) / run)};
-    pos += x.count;
   }
 };
 
@@ -337,7 +347,8 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
     long long x = 0;
     if (e < entries) {
       const int b = e / p.entries_per_seq;
-      x = static_cast<long long>(span_of(p, b, (e - b * p.entries_per_seq) * kCacheTcRows, kCacheTcRows).count) * p.mult;
+      const int count = span_of(p, b, (e - b * p.entries_per_seq) * kCacheTcRows, kCacheTcRows).count;
+      x = count > 0 ? static_cast<long long>(count + kItemCost) * p.mult : 0;
     }
     const long long own = x;
 #pragma unroll
@@ -474,16 +485,15 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           mask(va, 2 * half);
           mask(vb, 2 * half + 1);
         }
-        auto top = [&](const uint32_t(&v)[32], int c) {
-          float a = -INFINITY, a2 = -INFINITY;
+        float a0 = -INFINITY, a1 = -INFINITY, b0 = -INFINITY, b1 = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            a = fmaxf(a, __uint_as_float(v[i]));
-            a2 = fmaxf(a2, __uint_as_float(v[i + 1]));
-          }
-          return fmaf(fmaxf(a, a2), kc[c], ve[c]);
-        };
-        const float mx = fmaxf(top(va, 0), top(vb, 1));
+        for (int i = 0; i < 32; i += 4) {  // three-operand maxima in four chains
+          a0 = fmaxf(fmaxf(a0, __uint_as_float(va[i])), __uint_as_float(va[i + 1]));
+          b0 = fmaxf(fmaxf(b0, __uint_as_float(vb[i])), __uint_as_float(vb[i + 1]));
+          a1 = fmaxf(fmaxf(a1, __uint_as_float(va[i + 2])), __uint_as_float(va[i + 3]));
+          b1 = fmaxf(fmaxf(b1, __uint_as_float(vb[i + 2])), __uint_as_float(vb[i + 3]));
+        }
+        const float mx = fmaxf(fmaf(fmaxf(a0, a1), kc[0], ve[0]), fmaf(fmaxf(b0, b1), kc[1], ve[1]));
         const bool grow = mx > m + kRescaleThreshold;
         const bool scale_o = grow && n > 0 && m != -INFINITY;
         if (__any_sync(0xffffffffu, scale_o)) {
@@ -653,11 +663,22 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           raw[i] = row < n_keys ? load16(src + static_cast<long long>(row) * D) : make_uint4(0, 0, 0, 0);
         }
       };
+      // One thread asks for the tiles ahead in L2: the loads below are one tile ahead, which covers the
+      // latency of L2 and not that of HBM.
+      auto prefetch = [&](int base) {
+        const int rows = min(kKeys, n_keys - base);
+        if (c == 0 && rows > 0)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + static_cast<long long>(base) * D),
+                       "r"(rows * D)
+                       : "memory");
+      };
       load(0, NP, k0);
       float sc = scale_at(k0);
+      for (int i = 1; i < min(count, kAhead); ++i) prefetch(k0 + i * kKeys);
       for (int j = 0; j < count; ++j, ++tile_no, k0 += kKeys) {
         const int st = tile_no % NS;
         if (!(ok = mbar_wait_warp(&empty[st], ((tile_no / NS) & 1) ^ 1u, p.status, kTimeoutProducer, abort_flag))) break;
+        if (j + kAhead < count) prefetch(k0 + kAhead * kKeys);
         if (brings) {
           scales[st][c] = c < 4 ? sc : __log2f(sc);
           if (c >= 4) scales[st][4 + c] = 1.f / sc;
@@ -715,7 +736,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
     if (warp == kWalkWarp && lane == 0) {
       // ---------------------------------------------------------------- the run's pieces
-      const long long run = max((total + gridDim.x - 1) / gridDim.x, 2LL);
+      const long long run = max((total + gridDim.x - 1) / gridDim.x, 2LL + kItemCost);
       const long long from = min(blockIdx.x * run, total);
       walk.start(p, prefix, from, min(from + run, total), run);
       for (uint32_t seg = 0;; ++seg) {
