@@ -108,16 +108,13 @@ def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, interleave: bool =
     computed in fp32 and rounded once. On CUDA q and k take one kernel (bf16, fp16, fp32), and its
     transpose in the backward; factors that need a gradient take the torch operations.
     """
-    if use_native(q) and not interleave and q.dtype == torch.bfloat16 and cos.ndim == 3 and cos.shape[-1] * 2 == q.shape[-1]:
-        if cos.shape[-2] == 1:
-            from priml_b200.ops import functional
-
-            return functional.rotary(q, k, cos, sin)
     if use_native(q):
         from priml_b200.ops import functional
 
+        if not interleave and q.dtype == torch.bfloat16 and cos.ndim == 3 and cos.shape[-1] * 2 == q.shape[-1] and cos.shape[-2] == 1:
+            return functional.rotary(q, k, cos, sin)
         if functional.rotary_any_supported(q, k, cos, sin):
-            return functional.rotary_any(q, k, cos, sin, interleave)
+            return native().rotary(q, k, cos, sin, interleave)
     return reference.rotate(q, cos, sin, interleave), reference.rotate(k, cos, sin, interleave)
 
 
@@ -280,6 +277,8 @@ def rotary_append(
 
     On CUDA with bf16 and 64 or 128 channels a head this is one kernel (``csrc/rotary.cu``).
     """
+    if use_native(q) and q.dtype == k.dtype == v.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
+        return native().rotary_append(q, k, v, k_cache, v_cache, k_scale, v_scale, lengths, cos, sin, interleave)
     if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together.")
     if k.shape[2] != k_cache.shape[1]:
@@ -291,10 +290,6 @@ def rotary_append(
     _check_cache(q, k_cache, v_cache, k_scale, v_scale, lengths)
     if any(x.requires_grad for x in (q, k, v)) and torch.is_grad_enabled():
         raise RuntimeError("rotary_append has no gradient: call it under torch.no_grad().")
-    if use_native(q) and q.shape[-1] in (64, 128) and all(x.dtype == torch.bfloat16 for x in (q, k, v)):
-        return native().rotary_append(
-            q, k, v, k_cache, v_cache, k_scale, v_scale, lengths.to(torch.int32).contiguous(), cos, sin, interleave
-        )
     return reference.rotary_append(q, k, v, k_cache, v_cache, k_scale, v_scale, lengths, cos, sin, interleave)
 
 
@@ -321,28 +316,26 @@ def cache_attention(
 
     On CUDA with bf16 queries and 64 or 128 channels a head this runs ``csrc/cache_attention*.cu``.
     """
+    if window is not None and window < 0:
+        window = None
+    if not 0 <= offset < 1 << 31:
+        raise ValueError(f"offset must be a token count, got {offset}.")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if use_native(q) and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
+        return native().cache_attn(
+            q, k_cache, v_cache, k_scale, v_scale, lengths, offset, scale, -1 if window is None else int(window)
+        )
     if q.ndim not in (3, 4):
         raise ValueError(f"q must be [B, H, D] or [B, s, H, D], got {tuple(q.shape)}.")
     q4 = q[:, None] if q.ndim == 3 else q
     _check_cache(q4, k_cache, v_cache, k_scale, v_scale, lengths)
     if k_cache.shape[1] < 1 or q4.shape[2] % k_cache.shape[1]:
         raise ValueError(f"{q4.shape[2]} query heads are not a multiple of {k_cache.shape[1]} KV heads.")
-    if window is not None and window < 0:
-        window = None
-    if not 0 <= offset < 1 << 31:
-        raise ValueError(f"offset must be a token count, got {offset}.")
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("cache_attention has no gradient: call it under torch.no_grad().")
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if use_native(q) and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
-        out = native().cache_attn(
-            q4, k_cache, v_cache, k_scale, v_scale, lengths.to(torch.int32).contiguous(), offset, scale,
-            -1 if window is None else int(window),
-        )  # fmt: skip
-    else:
-        out = reference.cache_attention(
-            q4, k_cache, v_cache, k_scale, v_scale, lengths, scale=scale, window=window, offset=offset
-        )
+    out = reference.cache_attention(
+        q4, k_cache, v_cache, k_scale, v_scale, lengths, scale=scale, window=window, offset=offset
+    )
     return out[:, 0] if q.ndim == 3 else out
 
 

@@ -19,6 +19,7 @@ namespace {
 using torch::Tensor;
 
 #define PB_CHECK(cond, msg) TORCH_CHECK(cond, "priml_b200: ", msg)
+#define PB_VALUE(cond, msg) TORCH_CHECK_VALUE(cond, "priml_b200: ", msg)  // raises ValueError
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
@@ -757,29 +758,62 @@ std::vector<Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& cos, 
   return {qo, ko};
 }
 
+// The rotation with its gradient, the rotation by -sin (which is differentiable in turn). The autograd node
+// is C++: a training step makes one per attention layer and direction, and a Python node costs more host
+// time (about 45 us for a forward and backward, against 15 us) than the kernels take at most sizes.
+class RotaryFn : public torch::autograd::Function<RotaryFn> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const Tensor& cos, const Tensor& sin, bool interleave, double sign) {
+    ctx->save_for_backward({cos, sin});
+    ctx->saved_data["interleave"] = interleave;
+    ctx->saved_data["sign"] = sign;
+    return rotary(q.stride(3) == 1 ? q : q.contiguous(), k.stride(3) == 1 ? k : k.contiguous(), cos, sin, interleave, sign);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 const torch::autograd::variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleave = ctx->saved_data["interleave"].toBool();
+    const double sign = -ctx->saved_data["sign"].toDouble();
+    auto rows = [](const Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); };
+    auto d = at::GradMode::is_enabled() ? RotaryFn::apply(grads[0], grads[1], saved[0], saved[1], interleave, sign)
+                                        : rotary(rows(grads[0]), rows(grads[1]), saved[0], saved[1], interleave, sign);
+    return {d[0], d[1], Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary_fn(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
+                                     bool interleave) {
+  auto out = RotaryFn::apply(q, k, cos, sin, interleave, 1.0);
+  return {out[0], out[1]};
+}
+
 // The checks that the append and the attention share: an e4m3 cache [B, Hkv, T, D] with contiguous,
 // 16-byte aligned rows, and its fp32 scales [B, Hkv, ceil(T / 32)].
 void check_cache(const Tensor& cache, const Tensor& scale, const Tensor& ref, int64_t B, int64_t Hkv, int64_t T,
                  int64_t D, const char* name) {
   const std::string n(name);
-  PB_CHECK(cache.is_cuda() && cache.scalar_type() == torch::kFloat8_e4m3fn && cache.device() == ref.device(),
-           n + " cache must be float8_e4m3fn on the query's device");
-  PB_CHECK(cache.dim() == 4 && cache.size(0) == B && cache.size(1) == Hkv && cache.size(2) == T && cache.size(3) == D,
+  TORCH_CHECK_TYPE(cache.scalar_type() == torch::kFloat8_e4m3fn, "priml_b200: ", n, " cache must be float8_e4m3fn");
+  PB_VALUE(cache.device() == ref.device(), n + " cache must be on the query's device");
+  PB_VALUE(cache.dim() == 4 && cache.size(0) == B && cache.size(1) == Hkv && cache.size(2) == T && cache.size(3) == D,
            n + " cache must be [B, Hkv, T, D]");
-  PB_CHECK(cache.stride(3) == 1 && (cache.stride(2) == D || T <= 1), n + " cache rows must be contiguous");
-  PB_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0 && cache.stride(0) % 16 == 0 &&
+  PB_VALUE(cache.stride(3) == 1 && (cache.stride(2) == D || T <= 1), n + " cache rows must be contiguous");
+  PB_VALUE(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0 && cache.stride(0) % 16 == 0 &&
                cache.stride(1) % 16 == 0,
            n + " cache base and strides must be 16-byte aligned");
-  PB_CHECK(scale.is_cuda() && scale.scalar_type() == torch::kFloat32 && scale.device() == ref.device() &&
+  PB_VALUE(scale.is_cuda() && scale.scalar_type() == torch::kFloat32 && scale.device() == ref.device() &&
                scale.dim() == 3 && scale.size(0) == B && scale.size(1) == Hkv &&
                scale.size(2) == (T + pb::kCacheBlock - 1) / pb::kCacheBlock && (scale.stride(2) == 1 || scale.size(2) <= 1),
            n + " scales must be fp32 [B, Hkv, ceil(T / 32)] with contiguous blocks");
 }
 
-void check_lengths(const Tensor& lengths, const Tensor& ref, int64_t B) {
-  PB_CHECK(lengths.is_cuda() && lengths.device() == ref.device() && lengths.scalar_type() == torch::kInt32 &&
-               lengths.dim() == 1 && lengths.numel() == B && (lengths.stride(0) == 1 || B <= 1),
-           "lengths must be contiguous int32 [B] on the query's device");
+Tensor lengths_of(const Tensor& lengths, const Tensor& ref, int64_t B) {
+  PB_VALUE(lengths.device() == ref.device() && lengths.dim() == 1 && lengths.numel() == B &&
+               at::isIntegralType(lengths.scalar_type(), false),
+           "lengths must be integers [B] on the query's device");
+  if (lengths.scalar_type() == torch::kInt32 && lengths.is_contiguous()) return lengths;
+  const c10::cuda::CUDAGuard guard(ref.device());
+  return lengths.to(torch::kInt32).contiguous();
 }
 
 // A tensor the append writes must not map two of its (sequence, head) planes onto the same memory.
@@ -789,7 +823,7 @@ void check_planes(const Tensor& t, const char* name) {
   const int64_t sb = t.stride(0), sh = t.stride(1);
   const bool heads_in = h <= 1 || sh >= plane, seqs_in = b <= 1 || sb >= plane;
   const int64_t heads_span = h <= 1 ? plane : (h - 1) * sh + plane, seqs_span = b <= 1 ? plane : (b - 1) * sb + plane;
-  PB_CHECK(t.numel() == 0 || (heads_in && seqs_in && (b <= 1 || h <= 1 || sb >= heads_span || sh >= seqs_span)),
+  PB_VALUE(t.numel() == 0 || (heads_in && seqs_in && (b <= 1 || h <= 1 || sb >= heads_span || sh >= seqs_span)),
            std::string(name) + " must not overlap itself");
 }
 
@@ -803,33 +837,36 @@ Tensor rows16(const Tensor& t) {
 // Rotates q and k [B, s, H | Hkv, D] at positions lengths[b] + i (cos / sin: fp32 [P, R/2], or none) and
 // appends k and v to the 8-bit caches at those rows; returns the rotated q (q itself without factors).
 Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tensor& k_cache, Tensor& v_cache,
-                     Tensor& k_scale, Tensor& v_scale, const Tensor& lengths, const c10::optional<Tensor>& cos,
+                     Tensor& k_scale, Tensor& v_scale, const Tensor& lengths_, const c10::optional<Tensor>& cos,
                      const c10::optional<Tensor>& sin, bool interleave) {
   for (const Tensor* t : {&q_, &k_, &v_})
-    PB_CHECK(t->is_cuda() && t->scalar_type() == torch::kBFloat16 && t->dim() == 4 && t->device() == q_.device(),
+    PB_VALUE(t->is_cuda() && t->scalar_type() == torch::kBFloat16 && t->dim() == 4 && t->device() == q_.device(),
              "q, k and v must be bf16 [B, s, heads, D] on one device");
+  for (const Tensor* t : {&q_, &k_, &v_})
+    PB_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()),
+             "rotary_append has no gradient: call it under torch.no_grad()");
   const int64_t B = q_.size(0), s = q_.size(1), H = q_.size(2), D = q_.size(3), Hkv = k_.size(2);
-  PB_CHECK(D == 64 || D == 128, "the 8-bit cache covers head dims 64 and 128");
-  PB_CHECK(k_.sizes() == v_.sizes() && k_.size(0) == B && k_.size(1) == s && k_.size(3) == D,
+  PB_VALUE(D == 64 || D == 128, "the 8-bit cache covers head dims 64 and 128");
+  PB_VALUE(k_.sizes() == v_.sizes() && k_.size(0) == B && k_.size(1) == s && k_.size(3) == D,
            "k and v must be [B, s, Hkv, D] beside q");
-  PB_CHECK(k_cache.dim() == 4, "k cache must be [B, Hkv, T, D]");
+  PB_VALUE(k_cache.dim() == 4, "k cache must be [B, Hkv, T, D]");
   const int64_t T = k_cache.size(2);
   check_cache(k_cache, k_scale, q_, B, Hkv, T, D, "k");
   check_cache(v_cache, v_scale, q_, B, Hkv, T, D, "v");
-  check_lengths(lengths, q_, B);
+  const Tensor lengths = lengths_of(lengths_, q_, B);
   check_planes(k_cache, "k cache");
   check_planes(v_cache, "v cache");
   check_planes(k_scale, "k scales");
   check_planes(v_scale, "v scales");
-  PB_CHECK(cos.has_value() == sin.has_value(), "cos and sin come together");
-  PB_CHECK(T < (1LL << 31) - 64 && B * s < (1LL << 30) && B * Hkv * (s / pb::kCacheBlock + 2) < (1LL << 29),
+  PB_VALUE(cos.has_value() == sin.has_value(), "cos and sin come together");
+  PB_VALUE(T < (1LL << 31) - 64 && B * s < (1LL << 30) && B * Hkv * (s / pb::kCacheBlock + 2) < (1LL << 29),
            "sizes out of range");
   const c10::cuda::CUDAGuard guard(q_.device());
   auto q = rows16(q_), k = rows16(k_), v = rows16(v_);
   pb::AppendParams p{};
   Tensor c, n, out = q_;
   if (cos.has_value()) {
-    PB_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes() && cos->size(0) >= 1 && cos->size(1) >= 1 &&
+    PB_VALUE(cos->dim() == 2 && cos->sizes() == sin->sizes() && cos->size(0) >= 1 && cos->size(1) >= 1 &&
                  2 * cos->size(1) <= D,
              "cos and sin must be [positions, R/2] tables with R <= D");
     c = aux(*cos, q_, torch::kFloat32);
@@ -866,18 +903,22 @@ Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tenso
 // q [B, s, H, D] over 8-bit caches; query i of sequence b stands at position n - s + i with
 // n = min(lengths[b] + offset, T). Returns [B, s, H, D] (contiguous bf16).
 Tensor cache_attn(const Tensor& q_, const Tensor& k, const Tensor& v, const Tensor& k_scale, const Tensor& v_scale,
-                  const Tensor& lengths, int64_t offset, double scale, int64_t window) {
-  PB_CHECK(q_.is_cuda() && q_.scalar_type() == torch::kBFloat16 && q_.dim() == 4, "q must be CUDA bf16 [B, s, H, D]");
+                  const Tensor& lengths_, int64_t offset, double scale, int64_t window) {
+  if (q_.dim() == 3)
+    return cache_attn(q_.unsqueeze(1), k, v, k_scale, v_scale, lengths_, offset, scale, window).squeeze(1);
+  PB_VALUE(q_.is_cuda() && q_.scalar_type() == torch::kBFloat16 && q_.dim() == 4, "q must be CUDA bf16 [B, (s,) H, D]");
+  PB_CHECK(!(at::GradMode::is_enabled() && q_.requires_grad()),
+           "cache_attention has no gradient: call it under torch.no_grad()");
   const int64_t B = q_.size(0), s = q_.size(1), H = q_.size(2), D = q_.size(3);
-  PB_CHECK(D == 64 || D == 128, "the 8-bit cache covers head dims 64 and 128");
-  PB_CHECK(k.dim() == 4, "k cache must be [B, Hkv, T, D]");
+  PB_VALUE(D == 64 || D == 128, "the 8-bit cache covers head dims 64 and 128");
+  PB_VALUE(k.dim() == 4, "k cache must be [B, Hkv, T, D]");
   const int64_t Hkv = k.size(1), T = k.size(2);
   check_cache(k, k_scale, q_, B, Hkv, T, D, "k");
   check_cache(v, v_scale, q_, B, Hkv, T, D, "v");
-  check_lengths(lengths, q_, B);
-  PB_CHECK(Hkv > 0 && H % Hkv == 0, "query heads must be a multiple of the KV heads");
-  PB_CHECK(T < (1LL << 31) - 64 && s * (H / Hkv) < (1LL << 30) && B * s * H < (1LL << 31), "sizes out of range");
-  PB_CHECK(offset >= 0 && offset < (1LL << 31), "offset must be a token count");
+  const Tensor lengths = lengths_of(lengths_, q_, B);
+  PB_VALUE(Hkv > 0 && H % Hkv == 0, "query heads must be a multiple of the KV heads");
+  PB_VALUE(T < (1LL << 31) - 64 && s * (H / Hkv) < (1LL << 30) && B * s * H < (1LL << 31), "sizes out of range");
+  PB_VALUE(offset >= 0 && offset < (1LL << 31), "offset must be a token count");
   const c10::cuda::CUDAGuard guard(q_.device());
   auto q = rows16(q_);
   auto out = torch::empty({B, s, H, D}, q.options());
@@ -911,10 +952,9 @@ Tensor cache_attn(const Tensor& q_, const Tensor& k, const Tensor& v, const Tens
       p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()) + (b0 * s + s0) * H * D;
       long long part_floats = 0, plan_words = 0;
       pb::cache_attn_plan(p, static_cast<int>(D), &part_floats, &plan_words);
-      auto part = torch::empty({part_floats}, q.options().dtype(torch::kFloat32));
-      auto plan = torch::empty({plan_words}, q.options().dtype(torch::kInt64));
-      p.part = part.data_ptr<float>();
-      p.plan = reinterpret_cast<long long*>(plan.data_ptr<int64_t>());
+      auto work = torch::empty({part_floats + 2 * plan_words}, q.options().dtype(torch::kFloat32));
+      p.plan = reinterpret_cast<long long*>(work.data_ptr<float>());
+      p.part = work.data_ptr<float>() + 2 * plan_words;
       pb::cache_attn(p, static_cast<int>(D), stream());
     }
   }
@@ -1685,8 +1725,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q"), py::arg("c_kv"), py::arg("k_pe"), py::arg("lengths"), py::arg("scale"));
   m.def("decode_attn", &decode_attn, "one-token decode attention over a KV cache with device lengths",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("lengths"), py::arg("scale"), py::arg("window") = -1);
-  m.def("rotary", &rotary, "rotary embedding of q and k in any layout", py::arg("q"), py::arg("k"), py::arg("cos"),
-        py::arg("sin"), py::arg("interleave"), py::arg("sign"));
+  m.def("rotary", &rotary_fn, "rotary embedding of q and k in any layout, differentiable in q and k", py::arg("q"),
+        py::arg("k"), py::arg("cos"), py::arg("sin"), py::arg("interleave"));
   m.def("rotary_append", &rotary_append, "rotary embedding fused with the append to an 8-bit cache", py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"),
         py::arg("lengths"), py::arg("cos"), py::arg("sin"), py::arg("interleave"));

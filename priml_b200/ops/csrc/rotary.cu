@@ -187,68 +187,95 @@ __device__ __forceinline__ float of_e4m3(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
 }
 
-// The lane's N = D / 32 channels of one row, turned in fp32 when `cs` is given (the row's factors).
+// A lane's N = D / 32 channels of a row, and what turning them takes: each becomes x cs + other sn, with
+// `other` its pair's other channel and the sign of sin already in sn (the same products and the same
+// sum as `turn`). Channels at or past R keep their value.
 template <int N, bool INTER>
-__device__ __forceinline__ void load_turned(const __nv_bfloat16* row, int lane, int R, const float* cs, const float* sn,
-                                            float (&x)[N]) {
-  const int e0 = lane * N;
-  const Vec<__nv_bfloat16, N> raw = *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(row + e0);
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = to_f(raw.v[i]);
-  if (cs == nullptr || e0 >= R) return;
-  if (INTER) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      if (e0 + i < R) {
-        const int f = (e0 + i) >> 1;
-        float ya, yc;
-        turn(x[i], x[i + 1], cs[f], sn[f], ya, yc);
-        x[i] = ya;
-        x[i + 1] = yc;
-      }
-    }
-  } else {
-    const int half = R >> 1;
+struct Turner {
+  float cs[N], sn[N];
+  int shift;        // half-split layout: lanes between the channels of a pair
+  bool shuffled;    // a pair's channels lie at the same place of two lanes
+  bool upper;       // half-split layout: this lane holds second channels
+
+  __device__ __forceinline__ void factors(const float* cos, const float* sin, int lane, int R) {
+    const int e0 = lane * N, half = R >> 1;
+    shuffled = INTER || half % N == 0;
+    shift = half / N;
+    upper = e0 >= half;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = e0 + i;
-      if (e < R) {
-        const bool first = e < half;
-        const int f = first ? e : e - half;
-        const float other = to_f(row[first ? e + half : e - half]);
-        float ya, yc;
-        turn(first ? x[i] : other, first ? other : x[i], cs[f], sn[f], ya, yc);
-        x[i] = first ? ya : yc;
-      }
+      const bool first = INTER ? (i & 1) == 0 : e < half;
+      const int f = INTER ? e >> 1 : (first ? e : e - half);
+      cs[i] = e < R ? cos[f] : 1.f;
+      sn[i] = e < R ? (first ? -sin[f] : sin[f]) : 0.f;
     }
   }
+  // `row` is read again only where the pair's channels lie at different places of their lanes.
+  __device__ __forceinline__ void apply(float (&x)[N], const __nv_bfloat16* row, int lane, int R) const {
+    float other[N];
+    if (INTER) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) other[i] = x[i ^ 1];
+    } else if (shuffled) {
+      const int from = (upper ? lane - shift : lane + shift) & 31;
+#pragma unroll
+      for (int i = 0; i < N; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], from);
+    } else {
+      const int half = R >> 1;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = lane * N + i;
+        other[i] = e < R ? to_f(row[e < half ? e + half : e - half]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane * N + i < R) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(other[i], sn[i]));
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void load_row(const __nv_bfloat16* row, int lane, float (&x)[N]) {
+  const Vec<__nv_bfloat16, N> raw = *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(row + lane * N);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = to_f(raw.v[i]);
 }
 
-// CTAs [0, q_blocks) turn the queries, one token each (its heads over the four warps). The rest
-// take one (sequence, KV head, block of 32 cache rows, K or V) each: pass one leaves the rows'
-// values in registers and finds amax, pass two requantises old rows if need be and stores.
+// CTAs [0, q_blocks) turn the queries, one token each: its factors are read once, its heads go over the
+// four warps, eight rows in flight each. The rest take one (sequence, KV head, block of 32 cache rows, K
+// or V) each: pass one leaves the rows' values in registers and finds amax, pass two requantises old
+// rows if need be and stores.
 template <int D, bool INTER>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p) {
   constexpr int N = D / 32;
-  constexpr int kWarpRows = kRows / (kThreads / 32);
+  constexpr int kWarps = kThreads / 32;
+  constexpr int kWarpRows = kRows / kWarps;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long blk = blockIdx.x;
   if (blk < p.q_blocks) {
     const long long b = blk / p.s;
     const int i = static_cast<int>(blk - b * p.s);
-    const long long pos = min(max(static_cast<long long>(p.lengths[b]) + i, 0LL), p.table_rows - 1);
-    const float* cs = p.cos + pos * (p.R >> 1);
-    const float* sn = p.sin + pos * (p.R >> 1);
     const __nv_bfloat16* src = p.q + b * p.q_sb + i * p.q_ss;
     __nv_bfloat16* dst = p.q_out + blk * p.H * D;
-#pragma unroll 4
-    for (int h = warp; h < p.H; h += kThreads / 32) {
-      float x[N];
-      load_turned<N, INTER>(src + h * p.q_sh, lane, p.R, cs, sn, x);
-      Vec<__nv_bfloat16, N> y;
+    const long long pos = min(max(static_cast<long long>(p.lengths[b]) + i, 0LL), p.table_rows - 1);
+    Turner<N, INTER> turner;
+    turner.factors(p.cos + pos * (p.R >> 1), p.sin + pos * (p.R >> 1), lane, p.R);
+    for (int h0 = warp; h0 < p.H; h0 += 8 * kWarps) {
+      float x[8][N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) y.v[j] = from_f<__nv_bfloat16>(x[j]);
-      *reinterpret_cast<Vec<__nv_bfloat16, N>*>(dst + h * D + lane * N) = y;
+      for (int j = 0; j < 8; ++j)
+        if (h0 + j * kWarps < p.H) load_row<N>(src + (h0 + j * kWarps) * p.q_sh, lane, x[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int h = h0 + j * kWarps;
+        if (h >= p.H) break;
+        turner.apply(x[j], src + h * p.q_sh, lane, p.R);
+        Vec<__nv_bfloat16, N> y;
+#pragma unroll
+        for (int e = 0; e < N; ++e) y.v[e] = from_f<__nv_bfloat16>(x[j][e]);
+        *reinterpret_cast<Vec<__nv_bfloat16, N>*>(dst + static_cast<long long>(h) * D + lane * N) = y;
+      }
     }
     return;
   }
@@ -273,16 +300,25 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p)
   uint8_t* cache = (is_v ? p.v_cache + b * p.vc_sb + hk * p.vc_sh : p.k_cache + b * p.kc_sb + hk * p.kc_sh) + row0 * D;
   float* scale = (is_v ? p.v_scale + b * p.vs_sb + hk * p.vs_sh : p.k_scale + b * p.ks_sb + hk * p.ks_sh) + cb;
   const bool turn_it = !is_v && p.cos != nullptr;
+  const float held = lo > 0 ? *scale : 0.f;  // read before the barrier below, written after it
 
   float x[kWarpRows][N];
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < kWarpRows; ++j) {
-    const int r = warp + j * (kThreads / 32);
+    const int r = warp + j * kWarps;
+    if (r >= lo && r < hi) load_row<N>(x0 + (row0 + r - start) * x_ss, lane, x[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kWarpRows; ++j) {
+    const int r = warp + j * kWarps;
     if (r >= lo && r < hi) {
-      const long long pos = min(row0 + r, p.table_rows - 1);
-      load_turned<N, INTER>(x0 + (row0 + r - start) * x_ss, lane, p.R, turn_it ? p.cos + pos * (p.R >> 1) : nullptr,
-                            turn_it ? p.sin + pos * (p.R >> 1) : nullptr, x[j]);
+      if (turn_it) {
+        const long long pos = min(row0 + r, p.table_rows - 1);
+        Turner<N, INTER> turner;
+        turner.factors(p.cos + pos * (p.R >> 1), p.sin + pos * (p.R >> 1), lane, p.R);
+        turner.apply(x[j], x0 + (row0 + r - start) * x_ss, lane, p.R);
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float a = fabsf(x[j][i]);
@@ -290,20 +326,19 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p)
       }
     }
   }
-  const float held = lo > 0 ? *scale : 0.f;  // read before the barrier below, written after it
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  __shared__ float red[kThreads / 32];
+  __shared__ float red[kWarps];
   if (lane == 0) red[warp] = amax;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, red[w]);
+  for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, red[w]);
   const float now = fmaxf(block_scale(amax), held);
   const float inv = 1.f / now;
   if (threadIdx.x == 0) *scale = now;
 #pragma unroll
   for (int j = 0; j < kWarpRows; ++j) {
-    const int r = warp + j * (kThreads / 32);
+    const int r = warp + j * kWarps;
     if (r >= lo && r < hi) {
       Vec<uint8_t, N> y;
 #pragma unroll

@@ -407,27 +407,8 @@ class _Rotary(torch.autograd.Function):
         return n.rope(dq.contiguous(), c, s, -1.0), n.rope(dk.contiguous(), c, s, -1.0), None, None
 
 
-class _RotaryAny(torch.autograd.Function):
-    """Either pair layout, part of the head, factors per sequence or per head (``csrc/rotary.cu``).
-
-    The rotation is linear, and its transpose is the rotation by ``-sin``: the backward is this function again.
-    """
-
-    @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, interleave: bool, sign: float):  # type: ignore[override]
-        ctx.save_for_backward(cos, sin)
-        ctx.interleave, ctx.sign = interleave, sign
-        q, k = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k))
-        return tuple(native().rotary(q, k, cos, sin, interleave, sign))
-
-    @staticmethod
-    def backward(ctx, dq: Tensor, dk: Tensor):  # type: ignore[override]
-        cos, sin = ctx.saved_tensors
-        return *_RotaryAny.apply(dq, dk, cos, sin, ctx.interleave, -ctx.sign), None, None, None, None
-
-
 def rotary_any_supported(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> bool:
-    """Shapes and types that :class:`_RotaryAny` covers (factors that need a gradient do not)."""
+    """Shapes and types that ``csrc/rotary.cu`` covers (factors that need a gradient are not among them)."""
     return (
         q.ndim == 4
         and k.ndim == 4
@@ -449,10 +430,6 @@ def rotary_any_supported(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> bool
         and (cos.shape[-2] == 1 or cos.shape[-2] == q.shape[2] == k.shape[2])
         and not (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad))
     )
-
-
-def rotary_any(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, interleave: bool) -> tuple[Tensor, Tensor]:
-    return _RotaryAny.apply(q, k, cos.float(), sin.float(), interleave, 1.0)
 
 
 def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> tuple[Tensor, Tensor]:

@@ -331,14 +331,14 @@ def test_refusals_on_the_device() -> None:
         ops.cache_attention(q, k, v, ks, vs, n.cpu())
     with pytest.raises(ValueError, match="device"):
         ops.cache_attention(q, k.cpu(), v, ks, vs, n)
-    with pytest.raises(RuntimeError, match="contiguous"):  # rows with a stride of their own
+    with pytest.raises(ValueError, match="contiguous"):  # rows with a stride of their own
         wide = torch.zeros(2, 2, 64, 128, device="cuda").to(torch.float8_e4m3fn)
         ops.cache_attention(q, wide[..., :64], v, ks, vs, n)
-    with pytest.raises(RuntimeError, match="aligned"):
+    with pytest.raises(ValueError, match="aligned"):
         flat = torch.zeros(2 * 2 * 64 * 64 + 8, dtype=torch.uint8, device="cuda")[8:].view(torch.float8_e4m3fn)
         ops.cache_attention(q, flat.view(2, 2, 64, 64), v, ks, vs, n)
-    with pytest.raises(RuntimeError, match="overlap"):  # one cache for both sequences
+    with pytest.raises(ValueError, match="overlap"):  # one cache for both sequences
         ops.rotary_append(q, x, x, k[:1].expand(2, -1, -1, -1), v, ks, vs, n)
-    with pytest.raises(RuntimeError, match="overlap"):
+    with pytest.raises(ValueError, match="overlap"):
         ops.rotary_append(q, x, x, k, v, ks, vs[:, :1].expand(-1, 2, -1), n)
     assert ops.cache_attention(q, k[:1].expand(2, -1, -1, -1), v, ks, vs, n).shape == q.shape  # reading one is fine
