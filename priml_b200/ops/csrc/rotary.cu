@@ -187,28 +187,54 @@ __device__ __forceinline__ float of_e4m3(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
 }
 
+// max(m, |x|) that a NaN ends in.
+__device__ __forceinline__ float max_abs(float m, float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(x)));
+  return m;
+}
+
 // A lane's N = D / 32 channels of a row, and what turning them takes: each becomes x cs + other sn, with
 // `other` its pair's other channel and the sign of sin already in sn (the same products and the same
-// sum as `turn`). Channels at or past R keep their value.
-template <int N, bool INTER>
+// sum as `turn`). Channels at or past R keep their value. EASY: pairs lie at the same place of two lanes
+// (or in one lane), a lane is turned whole or not at all, and its factors can be read as one vector.
+template <int N, bool INTER, bool EASY>
 struct Turner {
   float cs[N], sn[N];
-  int shift;        // half-split layout: lanes between the channels of a pair
-  bool shuffled;    // a pair's channels lie at the same place of two lanes
-  bool upper;       // half-split layout: this lane holds second channels
+  int from;  // half-split layout: the lane that holds the pairs' other channels
 
   __device__ __forceinline__ void factors(const float* cos, const float* sin, int lane, int R) {
     const int e0 = lane * N, half = R >> 1;
-    shuffled = INTER || half % N == 0;
-    shift = half / N;
-    upper = e0 >= half;
+    if (EASY) {
+      const bool upper = !INTER && e0 >= half;
+      from = (upper ? lane - half / N : lane + half / N) & 31;
+      if (e0 >= R) return;
+      if (INTER) {
+        const Vec<float, N / 2> c = *reinterpret_cast<const Vec<float, N / 2>*>(cos + e0 / 2);
+        const Vec<float, N / 2> s = *reinterpret_cast<const Vec<float, N / 2>*>(sin + e0 / 2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = e0 + i;
-      const bool first = INTER ? (i & 1) == 0 : e < half;
-      const int f = INTER ? e >> 1 : (first ? e : e - half);
-      cs[i] = e < R ? cos[f] : 1.f;
-      sn[i] = e < R ? (first ? -sin[f] : sin[f]) : 0.f;
+        for (int i = 0; i < N; ++i) {
+          cs[i] = c.v[i / 2];
+          sn[i] = i & 1 ? s.v[i / 2] : -s.v[i / 2];
+        }
+      } else {
+        const int f = upper ? e0 - half : e0;
+        const Vec<float, N> c = *reinterpret_cast<const Vec<float, N>*>(cos + f);
+        const Vec<float, N> s = *reinterpret_cast<const Vec<float, N>*>(sin + f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          cs[i] = c.v[i];
+          sn[i] = upper ? s.v[i] : -s.v[i];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = e0 + i;
+        const bool first = INTER ? (i & 1) == 0 : e < half;
+        const int f = INTER ? e >> 1 : (first ? e : e - half);
+        cs[i] = e < R ? cos[f] : 1.f;
+        sn[i] = e < R ? (first ? -sin[f] : sin[f]) : 0.f;
+      }
     }
   }
   // `row` is read again only where the pair's channels lie at different places of their lanes.
@@ -217,8 +243,7 @@ struct Turner {
     if (INTER) {
 #pragma unroll
       for (int i = 0; i < N; ++i) other[i] = x[i ^ 1];
-    } else if (shuffled) {
-      const int from = (upper ? lane - shift : lane + shift) & 31;
+    } else if (EASY) {
 #pragma unroll
       for (int i = 0; i < N; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], from);
     } else {
@@ -229,15 +254,25 @@ struct Turner {
         other[i] = e < R ? to_f(row[e < half ? e + half : e - half]) : 0.f;
       }
     }
+    if (EASY) {
+      if (lane * N < R) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane * N + i < R) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(other[i], sn[i]));
+        for (int i = 0; i < N; ++i) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(other[i], sn[i]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (lane * N + i < R) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(other[i], sn[i]));
+    }
   }
 };
 
 template <int N>
-__device__ __forceinline__ void load_row(const __nv_bfloat16* row, int lane, float (&x)[N]) {
-  const Vec<__nv_bfloat16, N> raw = *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(row + lane * N);
+__device__ __forceinline__ Vec<__nv_bfloat16, N> load_row(const __nv_bfloat16* row, int lane) {
+  return *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(row + lane * N);
+}
+template <int N>
+__device__ __forceinline__ void widen(const Vec<__nv_bfloat16, N>& raw, float (&x)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = to_f(raw.v[i]);
 }
@@ -245,8 +280,9 @@ __device__ __forceinline__ void load_row(const __nv_bfloat16* row, int lane, flo
 // CTAs [0, q_blocks) turn the queries, one token each: its factors are read once, its heads go over the
 // four warps, eight rows in flight each. The rest take one (sequence, KV head, block of 32 cache rows, K
 // or V) each: pass one leaves the rows' values in registers and finds amax, pass two requantises old
-// rows if need be and stores.
-template <int D, bool INTER>
+// rows if need be and stores. What bounds it is the instructions per value next to 3 bytes of traffic, so
+// values are kept in vectors and the rare case (something not finite) in a branch of its own.
+template <int D, bool INTER, bool EASY>
 __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p) {
   constexpr int N = D / 32;
   constexpr int kWarps = kThreads / 32;
@@ -254,75 +290,91 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long blk = blockIdx.x;
   if (blk < p.q_blocks) {
-    const long long b = blk / p.s;
-    const int i = static_cast<int>(blk - b * p.s);
+    const int b = static_cast<int>(blk / p.s);
+    const int i = static_cast<int>(blk - static_cast<long long>(b) * p.s);
     const __nv_bfloat16* src = p.q + b * p.q_sb + i * p.q_ss;
     __nv_bfloat16* dst = p.q_out + blk * p.H * D;
     const long long pos = min(max(static_cast<long long>(p.lengths[b]) + i, 0LL), p.table_rows - 1);
-    Turner<N, INTER> turner;
+    Turner<N, INTER, EASY> turner;
     turner.factors(p.cos + pos * (p.R >> 1), p.sin + pos * (p.R >> 1), lane, p.R);
     for (int h0 = warp; h0 < p.H; h0 += 8 * kWarps) {
-      float x[8][N];
+      Vec<__nv_bfloat16, N> raw[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (h0 + j * kWarps < p.H) load_row<N>(src + (h0 + j * kWarps) * p.q_sh, lane, x[j]);
+        if (h0 + j * kWarps < p.H) raw[j] = load_row<N>(src + (h0 + j * kWarps) * p.q_sh, lane);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int h = h0 + j * kWarps;
         if (h >= p.H) break;
-        turner.apply(x[j], src + h * p.q_sh, lane, p.R);
+        float x[N];
+        widen<N>(raw[j], x);
+        turner.apply(x, src + h * p.q_sh, lane, p.R);
         Vec<__nv_bfloat16, N> y;
 #pragma unroll
-        for (int e = 0; e < N; ++e) y.v[e] = from_f<__nv_bfloat16>(x[j][e]);
-        *reinterpret_cast<Vec<__nv_bfloat16, N>*>(dst + static_cast<long long>(h) * D + lane * N) = y;
+        for (int e = 0; e < N; ++e) y.v[e] = from_f<__nv_bfloat16>(x[e]);
+        *reinterpret_cast<Vec<__nv_bfloat16, N>*>(dst + h * D + lane * N) = y;
       }
     }
     return;
   }
-  blk -= p.q_blocks;
-  const bool is_v = blk & 1;
-  blk >>= 1;
-  const int nth = static_cast<int>(blk % p.blocks_per_seq);
-  blk /= p.blocks_per_seq;
-  const int hk = static_cast<int>(blk % p.Hkv);
-  const long long b = blk / p.Hkv;
-  const long long start = p.lengths[b];               // first appended row
-  const long long end = min(start + p.s, static_cast<long long>(p.T));
-  if (start < 0) return;
-  const long long cb = start / kRows + nth;           // cache block
-  const long long row0 = cb * kRows;
-  const int lo = static_cast<int>(max(start - row0, 0LL));          // appended rows of the block: [lo, hi)
-  const int hi = static_cast<int>(min(end - row0, static_cast<long long>(kRows)));
+  unsigned rest = static_cast<unsigned>(blk - p.q_blocks);
+  const bool is_v = rest & 1;
+  rest >>= 1;
+  const int nth = static_cast<int>(rest % p.blocks_per_seq);
+  rest /= p.blocks_per_seq;
+  const int hk = static_cast<int>(rest % p.Hkv);
+  const int b = static_cast<int>(rest / p.Hkv);
+  const int start = p.lengths[b];                      // first appended row
+  if (start < 0 || start >= p.T) return;
+  const int end = static_cast<int>(min(static_cast<long long>(start) + p.s, static_cast<long long>(p.T)));
+  const int cb = start / kRows + nth;                  // cache block
+  const int row0 = cb * kRows;
+  const int lo = max(start - row0, 0);                 // appended rows of the block: [lo, hi)
+  const int hi = min(end - row0, kRows);
   if (hi <= lo) return;
 
-  const __nv_bfloat16* x0 = is_v ? p.v + b * p.v_sb + hk * p.v_sh : p.k + b * p.k_sb + hk * p.k_sh;
+  const __nv_bfloat16* x0 =
+      (is_v ? p.v + b * p.v_sb + hk * p.v_sh : p.k + b * p.k_sb + hk * p.k_sh) + (row0 - start) * (is_v ? p.v_ss : p.k_ss);
   const long long x_ss = is_v ? p.v_ss : p.k_ss;
-  uint8_t* cache = (is_v ? p.v_cache + b * p.vc_sb + hk * p.vc_sh : p.k_cache + b * p.kc_sb + hk * p.kc_sh) + row0 * D;
+  uint8_t* cache = (is_v ? p.v_cache + b * p.vc_sb + hk * p.vc_sh : p.k_cache + b * p.kc_sb + hk * p.kc_sh) +
+                   static_cast<long long>(row0) * D + lane * N;
   float* scale = (is_v ? p.v_scale + b * p.vs_sb + hk * p.vs_sh : p.k_scale + b * p.ks_sb + hk * p.ks_sh) + cb;
-  const bool turn_it = !is_v && p.cos != nullptr;
   const float held = lo > 0 ? *scale : 0.f;  // read before the barrier below, written after it
 
+  Vec<__nv_bfloat16, N> raw[kWarpRows];
+#pragma unroll
+  for (int j = 0; j < kWarpRows; ++j) {
+    const int r = warp + j * kWarps;
+    if (r >= lo && r < hi) raw[j] = load_row<N>(x0 + r * x_ss, lane);
+  }
   float x[kWarpRows][N];
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < kWarpRows; ++j) {
     const int r = warp + j * kWarps;
-    if (r >= lo && r < hi) load_row<N>(x0 + (row0 + r - start) * x_ss, lane, x[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < kWarpRows; ++j) {
-    const int r = warp + j * kWarps;
     if (r >= lo && r < hi) {
-      if (turn_it) {
-        const long long pos = min(row0 + r, p.table_rows - 1);
-        Turner<N, INTER> turner;
-        turner.factors(p.cos + pos * (p.R >> 1), p.sin + pos * (p.R >> 1), lane, p.R);
-        turner.apply(x[j], x0 + (row0 + r - start) * x_ss, lane, p.R);
+      widen<N>(raw[j], x[j]);
+      if (!is_v && p.cos != nullptr) {
+        const long long at = min(static_cast<long long>(row0 + r), p.table_rows - 1) * (p.R >> 1);
+        Turner<N, INTER, EASY> turner;
+        turner.factors(p.cos + at, p.sin + at, lane, p.R);
+        turner.apply(x[j], x0 + r * x_ss, lane, p.R);
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float a = fabsf(x[j][i]);
-        if (a < INFINITY) amax = fmaxf(amax, a);  // false for NaN too
+      for (int i = 0; i < N; ++i) amax = max_abs(amax, x[j][i]);
+    }
+  }
+  // (a block with something that is not finite in it finds its scale again, without that)
+  if (__syncthreads_or(!(amax < INFINITY))) {
+    amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < kWarpRows; ++j) {
+      const int r = warp + j * kWarps;
+      if (r >= lo && r < hi) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (fabsf(x[j][i]) < INFINITY) amax = fmaxf(amax, fabsf(x[j][i]));
+          else x[j][i] = NAN;
       }
     }
   }
@@ -340,12 +392,14 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p)
   for (int j = 0; j < kWarpRows; ++j) {
     const int r = warp + j * kWarps;
     if (r >= lo && r < hi) {
-      Vec<uint8_t, N> y;
+      // (NaN converts to NaN; everything else is within +-448 now)
+      Vec<uint16_t, N / 2> y;
 #pragma unroll
-      for (int i = 0; i < N; ++i) y.v[i] = static_cast<uint8_t>(e4m3_of(x[j][i] * inv));
-      *reinterpret_cast<Vec<uint8_t, N>*>(cache + r * D + lane * N) = y;
+      for (int i = 0; i < N; i += 2)
+        y.v[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(x[j][i] * inv, x[j][i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      *reinterpret_cast<Vec<uint16_t, N / 2>*>(cache + r * D) = y;
     } else if (r < lo && now > held) {
-      Vec<uint8_t, N>* at = reinterpret_cast<Vec<uint8_t, N>*>(cache + r * D + lane * N);
+      Vec<uint8_t, N>* at = reinterpret_cast<Vec<uint8_t, N>*>(cache + r * D);
       Vec<uint8_t, N> y = *at;
       const float f = held * inv;
 #pragma unroll
@@ -371,16 +425,20 @@ void rotary_append(AppendParams p, int D, bool interleave, cudaStream_t stream) 
   p.blocks_per_seq = p.s == 1 ? 1 : (p.s - 1 + kRows - 1) / kRows + 1;
   const long long blocks = p.q_blocks + 2LL * p.B * p.Hkv * p.blocks_per_seq;
   const unsigned grid = static_cast<unsigned>(blocks);
+  const int N = D / 32, half = p.R >> 1;
+  const bool aligned = reinterpret_cast<uintptr_t>(p.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sin) % 16 == 0;
+  const bool easy = aligned && (interleave ? p.R % N == 0 && (half * 2) % N == 0 : half % N == 0);
+  auto run = [&](auto kern) { kern<<<grid, kThreads, 0, stream>>>(p); };
   if (D == 64) {
     if (interleave)
-      rotary_append_kernel<64, true><<<grid, kThreads, 0, stream>>>(p);
+      easy ? run(rotary_append_kernel<64, true, true>) : run(rotary_append_kernel<64, true, false>);
     else
-      rotary_append_kernel<64, false><<<grid, kThreads, 0, stream>>>(p);
+      easy ? run(rotary_append_kernel<64, false, true>) : run(rotary_append_kernel<64, false, false>);
   } else {
     if (interleave)
-      rotary_append_kernel<128, true><<<grid, kThreads, 0, stream>>>(p);
+      easy ? run(rotary_append_kernel<128, true, true>) : run(rotary_append_kernel<128, true, false>);
     else
-      rotary_append_kernel<128, false><<<grid, kThreads, 0, stream>>>(p);
+      easy ? run(rotary_append_kernel<128, false, true>) : run(rotary_append_kernel<128, false, false>);
   }
 }
 
