@@ -382,9 +382,8 @@ struct RotaryParams {
   int S, H, Hk, D, R;
   float sign;        // -1: the transposed rotation (the gradient)
   int interleave;
-  int tokens_per_block;  // set by the launcher
 };
-void rotary(RotaryParams p, int dtype, cudaStream_t stream);
+void rotary(const RotaryParams& p, int dtype, cudaStream_t stream);
 
 // 8-bit caches: e4m3 rows with one power-of-two scale per kCacheBlock rows and head.
 constexpr int kCacheBlock = 32;

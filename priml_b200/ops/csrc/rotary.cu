@@ -55,97 +55,112 @@ __device__ __forceinline__ void turn(float a, float c, float cs, float sn, float
   yc = __fadd_rn(__fmul_rn(c, cs), __fmul_rn(a, sn));
 }
 
-// One thread turns (or copies) 2 V channels of one head: two vectors of V elements each.
-// Units of a head: R / (2V) turned ones, then (D - R) / (2V) copied ones.
+// Division of n < 2^31 by a number known at launch: floor(n / d) = (umulhi(m, n) + n) >> l with
+// l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1 (Granlund and Montgomery 1994).
+struct Divider {
+  uint32_t mul, shift, by;
+  explicit Divider(uint32_t d) : shift(0), by(d) {
+    while ((1ull << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(mul, n) + n) >> shift; }
+};
+
+// One thread turns (or copies) a unit: 2 V channels of one head, two vectors of V elements. A head has
+// R / (2V) turned ones, then (D - R) / (2V) copied ones. Bound by the bytes in flight: eight blocks per SM
+// (32 registers) with one unit per thread move 335 MB in 58 us (5.8 TB/s); two units per thread 72 us, four
+// 105 us.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
-  const int units = p.D / (2 * V);
+__global__ void __launch_bounds__(256, 8) rotary_kernel(RotaryParams p, Divider per_token, Divider per_head, Divider per_seq,
+                                                        uint32_t total) {
+  const uint32_t w = blockIdx.x * 256u + threadIdx.x;
+  if (w >= total) return;
   const int turned = p.R / (2 * V);
-  const int heads = p.H + p.Hk;
-  const int per_token = heads * units;
-  const long long tok0 = static_cast<long long>(blockIdx.x) * p.tokens_per_block;
-  const int ntok = static_cast<int>(min(static_cast<long long>(p.tokens_per_block), p.tokens - tok0));
-  for (int w = threadIdx.x; w < ntok * per_token; w += blockDim.x) {
-    const int lt = w / per_token;
-    const int r = w - lt * per_token;
-    const int h = r / units;
-    const int u = r - h * units;
-    const long long tok = tok0 + lt;
-    const long long b = tok / p.S;
-    const long long s = tok - b * p.S;
-    const bool is_q = h < p.H;
-    const int hh = is_q ? h : h - p.H;
-    const T* src = is_q ? static_cast<const T*>(p.q) + b * p.q_sb + s * p.q_ss + hh * p.q_sh
-                        : static_cast<const T*>(p.k) + b * p.k_sb + s * p.k_ss + hh * p.k_sh;
-    T* dst = is_q ? static_cast<T*>(p.q_out) + (tok * p.H + hh) * p.D : static_cast<T*>(p.k_out) + (tok * p.Hk + hh) * p.D;
-    int e0, e1;  // first channels of the thread's two vectors
-    if (u >= turned) {
-      e0 = p.R + (u - turned) * 2 * V;
-      e1 = e0 + V;
-    } else if (INTER) {
-      e0 = u * 2 * V;
-      e1 = e0 + V;
-    } else {
-      e0 = u * V;
-      e1 = e0 + p.R / 2;
-    }
-    const Vec<T, V> x0 = *reinterpret_cast<const Vec<T, V>*>(src + e0);
-    const Vec<T, V> x1 = *reinterpret_cast<const Vec<T, V>*>(src + e1);
-    Vec<T, V> y0 = x0, y1 = x1;
-    if (u < turned) {
-      const long long at = b * p.f_sb + s * p.f_ss + (p.f_sh == 0 ? 0 : hh * p.f_sh) + u * V;
-      float cs[V], sn[V];
+  const uint32_t tok = per_token.div(w), r = w - tok * per_token.by;
+  const int h = per_head.div(r), u = r - h * per_head.by;
+  const uint32_t b = per_seq.div(tok), s = tok - b * per_seq.by;
+  const bool is_q = h < p.H;
+  const int hh = is_q ? h : h - p.H;
+  const T* src = is_q ? static_cast<const T*>(p.q) + b * p.q_sb + s * p.q_ss + hh * p.q_sh
+                      : static_cast<const T*>(p.k) + b * p.k_sb + s * p.k_ss + hh * p.k_sh;
+  T* dst = is_q ? static_cast<T*>(p.q_out) + (static_cast<long long>(tok) * p.H + hh) * p.D
+                : static_cast<T*>(p.k_out) + (static_cast<long long>(tok) * p.Hk + hh) * p.D;
+  int e0, e1;  // first channels of the unit's two vectors
+  if (u >= turned) {
+    e0 = p.R + (u - turned) * 2 * V;
+    e1 = e0 + V;
+  } else if (INTER) {
+    e0 = u * 2 * V;
+    e1 = e0 + V;
+  } else {
+    e0 = u * V;
+    e1 = e0 + p.R / 2;
+  }
+  const Vec<T, V> x0 = *reinterpret_cast<const Vec<T, V>*>(src + e0);
+  const Vec<T, V> x1 = *reinterpret_cast<const Vec<T, V>*>(src + e1);
+  Vec<T, V> y0 = x0, y1 = x1;
+  if (u < turned) {
+    const long long at = b * p.f_sb + s * p.f_ss + hh * p.f_sh + u * V;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        cs[i] = p.cos[at + i];
-        sn[i] = p.sign * p.sin[at + i];
-      }
+    for (int i = 0; i < V; ++i) {
+      const float cs = p.cos[at + i], sn = p.sign * p.sin[at + i];
+      float ya, yc;
       if (INTER) {
         // pair i of the unit: channels 2i and 2i + 1 of its 2V contiguous ones
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float a = to_f(2 * i < V ? x0.v[(2 * i) % V] : x1.v[(2 * i) % V]);
-          const float c = to_f(2 * i + 1 < V ? x0.v[(2 * i + 1) % V] : x1.v[(2 * i + 1) % V]);
-          float ya, yc;
-          turn(a, c, cs[i], sn[i], ya, yc);
-          if (2 * i < V)
-            y0.v[(2 * i) % V] = from_f<T>(ya);
-          else
-            y1.v[(2 * i) % V] = from_f<T>(ya);
-          if (2 * i + 1 < V)
-            y0.v[(2 * i + 1) % V] = from_f<T>(yc);
-          else
-            y1.v[(2 * i + 1) % V] = from_f<T>(yc);
-        }
+        constexpr int W = V;
+        const int a = 2 * i, c = 2 * i + 1;
+        turn(to_f(a < W ? x0.v[a % W] : x1.v[a % W]), to_f(c < W ? x0.v[c % W] : x1.v[c % W]), cs, sn, ya, yc);
+        if (a < W)
+          y0.v[a % W] = from_f<T>(ya);
+        else
+          y1.v[a % W] = from_f<T>(ya);
+        if (c < W)
+          y0.v[c % W] = from_f<T>(yc);
+        else
+          y1.v[c % W] = from_f<T>(yc);
       } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float ya, yc;
-          turn(to_f(x0.v[i]), to_f(x1.v[i]), cs[i], sn[i], ya, yc);
-          y0.v[i] = from_f<T>(ya);
-          y1.v[i] = from_f<T>(yc);
-        }
+        turn(to_f(x0.v[i]), to_f(x1.v[i]), cs, sn, ya, yc);
+        y0.v[i] = from_f<T>(ya);
+        y1.v[i] = from_f<T>(yc);
       }
     }
-    *reinterpret_cast<Vec<T, V>*>(dst + e0) = y0;
-    *reinterpret_cast<Vec<T, V>*>(dst + e1) = y1;
   }
+  *reinterpret_cast<Vec<T, V>*>(dst + e0) = y0;
+  *reinterpret_cast<Vec<T, V>*>(dst + e1) = y1;
 }
 
 template <typename T, int V>
-void launch_rotary_v(RotaryParams& p, cudaStream_t stream) {
-  const int per_token = (p.H + p.Hk) * (p.D / (2 * V));
-  p.tokens_per_block = per_token >= 256 ? 1 : 256 / per_token;
-  const long long blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  if (p.interleave)
-    rotary_kernel<T, V, true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-  else
-    rotary_kernel<T, V, false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+void launch_rotary_v(const RotaryParams& all, cudaStream_t stream) {
+  const uint32_t units = all.D / (2 * V), per_token = (all.H + all.Hk) * units;
+  // whole sequences per launch (or part of one, with its own base pointers), so that unit counts stay within 2^30
+  const long long most = (1LL << 30) / per_token;
+  const long long B = all.tokens / all.S;
+  const long long seqs = most / all.S > 0 ? most / all.S : 1;
+  const long long toks = seqs * all.S <= most ? all.S : most;
+  for (long long b0 = 0; b0 < B; b0 += seqs) {
+    for (long long s0 = 0; s0 < all.S; s0 += toks) {
+      RotaryParams p = all;
+      const long long nb = B - b0 < seqs ? B - b0 : seqs, ns = all.S - s0 < toks ? all.S - s0 : toks;
+      p.q = static_cast<const T*>(all.q) + b0 * all.q_sb + s0 * all.q_ss;
+      p.k = static_cast<const T*>(all.k) + b0 * all.k_sb + s0 * all.k_ss;
+      p.q_out = static_cast<T*>(all.q_out) + (b0 * all.S + s0) * all.H * all.D;
+      p.k_out = static_cast<T*>(all.k_out) + (b0 * all.S + s0) * all.Hk * all.D;
+      p.cos += b0 * all.f_sb + s0 * all.f_ss;
+      p.sin += b0 * all.f_sb + s0 * all.f_ss;
+      const uint32_t total = static_cast<uint32_t>(nb * ns * per_token);
+      const unsigned grid = (total + 255) / 256;
+      const Divider dt(per_token), dh(units), ds(static_cast<uint32_t>(ns));
+      if (p.interleave)
+        rotary_kernel<T, V, true><<<grid, 256, 0, stream>>>(p, dt, dh, ds, total);
+      else
+        rotary_kernel<T, V, false><<<grid, 256, 0, stream>>>(p, dt, dh, ds, total);
+    }
+  }
 }
 
 // Widest vector that the channel counts, strides and base addresses all allow.
 template <typename T>
-void launch_rotary(RotaryParams& p, cudaStream_t stream) {
+void launch_rotary(const RotaryParams& p, cudaStream_t stream) {
   auto fits = [&](int v) {
     const long long bytes = static_cast<long long>(v) * sizeof(T);
     if (p.D % (2 * v) != 0 || p.R % (2 * v) != 0) return false;
@@ -283,7 +298,7 @@ __device__ __forceinline__ void widen(const Vec<__nv_bfloat16, N>& raw, float (&
 // rows if need be and stores. What bounds it is the instructions per value next to 3 bytes of traffic, so
 // values are kept in vectors and the rare case (something not finite) in a branch of its own.
 template <int D, bool INTER, bool EASY>
-__global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 7) rotary_append_kernel(AppendParams p) {
   constexpr int N = D / 32;
   constexpr int kWarps = kThreads / 32;
   constexpr int kWarpRows = kRows / kWarps;
@@ -411,7 +426,7 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(AppendParams p)
 
 }  // namespace
 
-void rotary(RotaryParams p, int dtype, cudaStream_t stream) {
+void rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
   if (dtype == 0)
     launch_rotary<__nv_bfloat16>(p, stream);
   else if (dtype == 1)
