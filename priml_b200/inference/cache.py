@@ -22,6 +22,13 @@ rows ``lengths[b] + i`` and attends over the visible rows:
 
 Rows past ``T`` are not written (the index is clamped to the last row); the
 decoder tracks lengths on the host as well and refuses to overflow.
+
+:class:`Fp8KVCache` is the same cache in 8 bits: e4m3 rows with one power-of-two scale
+per 32 rows and head, half the bytes that a decode step reads. It rotates queries and
+keys itself, from a table of the capacity's positions, in the kernel that quantises and
+appends them, and attends over the cache for prompts, chunks and single tokens alike, so
+what a token sees does not depend on how its prompt was cut (but for the scales of a
+block that fills in several calls).
 """
 
 from __future__ import annotations
@@ -34,7 +41,7 @@ from torch import Tensor
 
 from priml_b200 import ops
 
-__all__ = ["CacheState", "StaticKVCache"]
+__all__ = ["CacheState", "Fp8KVCache", "StaticKVCache"]
 
 
 @dataclass
@@ -126,3 +133,62 @@ class StaticKVCache:
         out = F.scaled_dot_product_attention(q.transpose(1, 2), kf.to(q.dtype), vf.to(q.dtype), attn_mask=ok[:, None],
                                              scale=scale)  # fmt: skip
         return out.transpose(1, 2)
+
+
+class Fp8KVCache:
+    """8-bit key/value buffers of one attention layer: ``[B, Hkv, T, D]`` e4m3 rows and their scales."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "state", "cos", "sin")
+
+    def __init__(
+        self,
+        k: Tensor,
+        v: Tensor,
+        k_scale: Tensor,
+        v_scale: Tensor,
+        state: CacheState,
+        cos: Tensor | None = None,
+        sin: Tensor | None = None,
+    ) -> None:
+        self.k, self.v, self.k_scale, self.v_scale, self.state = k, v, k_scale, v_scale, state
+        self.cos, self.sin = cos, sin
+
+    @classmethod
+    def alloc(
+        cls,
+        state: CacheState,
+        *,
+        heads: int,
+        channels_head: int,
+        device: torch.device | str | None = None,
+        cos: Tensor | None = None,
+        sin: Tensor | None = None,
+    ) -> Fp8KVCache:
+        """An empty cache; ``cos`` / ``sin`` (``[T, R/2]``) make it rotate what it appends and attends with."""
+        b, t = state.lengths.shape[0], state.capacity
+        if cos is not None and cos.shape[0] < t:
+            raise ValueError(f"{cos.shape[0]} rotary positions for a cache of {t} rows.")
+        k, v = (torch.zeros(b, heads, t, channels_head, device=device, dtype=torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.ones(b, heads, -(-t // ops.CACHE_BLOCK), device=device) for _ in range(2))
+        return cls(k, v, ks, vs, state, cos, sin)
+
+    def select(self, rows: slice, state: CacheState) -> Fp8KVCache:
+        return Fp8KVCache(
+            self.k[rows], self.v[rows], self.k_scale[rows], self.v_scale[rows], state, self.cos, self.sin
+        )
+
+    @property
+    def rotates(self) -> bool:
+        """Whether :meth:`attend` takes queries and keys that are not rotated yet."""
+        return self.cos is not None
+
+    @property
+    def seen(self) -> int:
+        raise RuntimeError("an 8-bit cache keeps its lengths on the device; pass positions explicitly")
+
+    def attend(self, q: Tensor, k: Tensor, v: Tensor, *, scale: float | None = None, window: int = -1) -> Tensor:
+        """Append ``[B, s, Hkv, D]`` keys/values and attend ``[B, s, H, D]`` queries; returns ``[B, s, H, D]``."""
+        cache = (self.k, self.v, self.k_scale, self.v_scale, self.state.lengths)
+        q = ops.rotary_append(q, k, v, *cache, cos=self.cos, sin=self.sin)
+        win = None if window is None or window < 0 else int(window)
+        return ops.cache_attention(q, *cache, scale=scale, window=win, offset=q.shape[1])

@@ -34,8 +34,9 @@ from typing import Any
 import torch
 from torch import Tensor, nn
 
-from priml_b200.inference.cache import CacheState, StaticKVCache
+from priml_b200.inference.cache import CacheState, Fp8KVCache, StaticKVCache
 from priml_b200.inference.sampling import SamplingParams, sample
+from priml_b200.models.rope import RoPE
 
 __all__ = ["Decoder"]
 
@@ -57,8 +58,11 @@ class Decoder:
         batch: int,
         max_seq: int,
         dtype: torch.dtype | None = None,
+        kv_dtype: torch.dtype | None = None,
         cuda_graph: bool = True,
     ) -> None:
+        """``kv_dtype=torch.float8_e4m3fn`` keeps keys and values in 8 bits (:class:`Fp8KVCache`); by default
+        they have the activations' ``dtype``."""
         from priml_b200.models.attention import SelfAttention
 
         blocks = list(getattr(model, "blocks", []))
@@ -69,11 +73,10 @@ class Decoder:
         self.dtype = dtype or _param_dtype(model)
         self.batch, self.max_seq = batch, max_seq
         self.state = CacheState.create(batch, max_seq, self.device)
-        self.caches = [
-            StaticKVCache.alloc(self.state, heads=b.attn.num_heads_kv, channels_head=b.attn.channels_head,
-                                device=self.device, dtype=self.dtype)  # fmt: skip
-            for b in blocks
-        ]
+        if kv_dtype not in (None, self.dtype, torch.float8_e4m3fn):
+            raise ValueError(f"kv_dtype must be {self.dtype} or torch.float8_e4m3fn, got {kv_dtype}.")
+        make = self._fp8_cache if kv_dtype == torch.float8_e4m3fn else self._static_cache
+        self.caches: list[StaticKVCache | Fp8KVCache] = [make(b.attn) for b in blocks]
         self.host_lengths = [0] * batch
         self.use_graph = cuda_graph and self.device.type == "cuda"
         self._tok = torch.zeros(batch, dtype=torch.long, device=self.device)
@@ -81,6 +84,17 @@ class Decoder:
         self._top_k = torch.zeros(batch, dtype=torch.long, device=self.device)
         self._top_p = torch.ones(batch, dtype=torch.float32, device=self.device)
         self._graphs: dict[bool, tuple[torch.cuda.CUDAGraph, Tensor, Tensor]] = {}
+
+    def _static_cache(self, attn: Any) -> StaticKVCache:
+        return StaticKVCache.alloc(self.state, heads=attn.num_heads_kv, channels_head=attn.channels_head,
+                                   device=self.device, dtype=self.dtype)  # fmt: skip
+
+    def _fp8_cache(self, attn: Any) -> Fp8KVCache:
+        cos = sin = None
+        if type(attn.rope) is RoPE:  # factors of other embeddings are the module's to apply
+            cos, sin = (f[:, 0].float().contiguous() for f in attn.rope.table(self.max_seq, self.device))
+        return Fp8KVCache.alloc(self.state, heads=attn.num_heads_kv, channels_head=attn.channels_head,
+                                device=self.device, cos=cos, sin=sin)  # fmt: skip
 
     # ------------------------------------------------------------------ state
     def reset(self, rows: slice | None = None) -> None:
@@ -104,7 +118,7 @@ class Decoder:
     _filtered = False
 
     # ------------------------------------------------------------------ forward
-    def _forward(self, tokens: Tensor, state: CacheState, caches: list[StaticKVCache]) -> Tensor:
+    def _forward(self, tokens: Tensor, state: CacheState, caches: list[StaticKVCache | Fp8KVCache]) -> Tensor:
         model: Any = self.model
         s = tokens.shape[1]
         x = model.embed(tokens)

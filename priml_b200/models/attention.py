@@ -341,7 +341,10 @@ class SelfAttention(nn.Module):
             q = self.norm_q(q)
         if self.norm_k is not None:
             k = self.norm_k(k)
-        if cos_sin is not None:
+        if getattr(cache, "rotates", False):
+            if cos_sin is not None:
+                raise ValueError("this cache rotates queries and keys itself; cos_sin cannot be passed with it.")
+        elif cos_sin is not None:
             q, k = RoPE.rotate(q, k, *cos_sin)
         elif self.rope is not None:
             if positions is None and cache is None and type(self.rope) is RoPE:

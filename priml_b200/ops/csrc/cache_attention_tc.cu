@@ -49,7 +49,6 @@ static_assert(256 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsIssue <= kLau
 constexpr int kGroupBarrier = 1;  // named barrier of the softmax warps
 constexpr float kShift = 7.f;     // weights are up to 2^(threshold + shift) = 2^15, within f16
 constexpr int kItemCost = 3;       // an item's start and end cost a CTA about as much as this many key tiles
-constexpr int kAhead = 6;          // key tiles that are asked for in L2 before their loads
 constexpr int kPolyOf4 = 1;       // of four pairs of weights this one takes exp2_poly
 constexpr int kPieces = 4;        // work pieces in flight between the walking warp and the others
 constexpr int kScratchCols = 32;  // columns that the groups exchange at a time
@@ -475,12 +474,17 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
             uint32_t bad = 0;
 #pragma unroll
             for (int w = 0; w < kConvertWarps; ++w) bad |= v_bad[st][w][c];
+            // bit i: the row sees key i of these
+            const int hi = kmax - k0 - 32 * c, lo = kmin - k0 - 32 * c;
+            const uint32_t sees = (hi < 0 ? 0u : hi > 30 ? ~0u : (2u << hi) - 1u) & (lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo);
+            if (bad != 0) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int key = k0 + 32 * c + i;
-              if (bad >> i & 1) v[i] = 0x7fffffffu;
-              if (key > kmax || key < kmin) v[i] = __float_as_uint(-INFINITY);
+              for (int i = 0; i < 32; ++i)
+                if (bad >> i & 1) v[i] = 0x7fffffffu;
             }
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(sees >> i & 1)) v[i] = __float_as_uint(-INFINITY);
           };
           mask(va, 2 * half);
           mask(vb, 2 * half + 1);
@@ -663,22 +667,11 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           raw[i] = row < n_keys ? load16(src + static_cast<long long>(row) * D) : make_uint4(0, 0, 0, 0);
         }
       };
-      // One thread asks for the tiles ahead in L2: the loads below are one tile ahead, which covers the
-      // latency of L2 and not that of HBM.
-      auto prefetch = [&](int base) {
-        const int rows = min(kKeys, n_keys - base);
-        if (c == 0 && rows > 0)
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + static_cast<long long>(base) * D),
-                       "r"(rows * D)
-                       : "memory");
-      };
       load(0, NP, k0);
       float sc = scale_at(k0);
-      for (int i = 1; i < min(count, kAhead); ++i) prefetch(k0 + i * kKeys);
       for (int j = 0; j < count; ++j, ++tile_no, k0 += kKeys) {
         const int st = tile_no % NS;
         if (!(ok = mbar_wait_warp(&empty[st], ((tile_no / NS) & 1) ^ 1u, p.status, kTimeoutProducer, abort_flag))) break;
-        if (j + kAhead < count) prefetch(k0 + kAhead * kKeys);
         if (brings) {
           scales[st][c] = c < 4 ? sc : __log2f(sc);
           if (c >= 4) scales[st][4 + c] = 1.f / sc;

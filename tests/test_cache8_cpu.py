@@ -154,3 +154,72 @@ def test_empty_batches_and_chunks() -> None:
     e = torch.zeros(2, 0, 2, 16)
     assert ops.rotary_append(torch.zeros(2, 0, 4, 16), e, e, k, v, ks, vs, n).shape == (2, 0, 4, 16)
     assert reference.CACHE_BLOCK == BLOCK == ops.CACHE_BLOCK
+
+
+# --------------------------------------------------------------------------- the cache in a decoder
+def _decoders(batch: int, max_seq: int):  # noqa: ANN202
+    from priml_b200.inference import Decoder
+    from priml_b200.models.presets import tiny_lm
+
+    torch.manual_seed(0)
+    model = tiny_lm().make().eval()
+    return Decoder(model, batch=batch, max_seq=max_seq), Decoder(
+        model, batch=batch, max_seq=max_seq, kv_dtype=torch.float8_e4m3fn
+    )
+
+
+def test_decoder_with_an_8_bit_cache_holds_the_rounded_keys() -> None:
+    full, small = _decoders(2, 96)
+    prompt = torch.randint(0, 512, (2, 45), generator=torch.Generator().manual_seed(1))
+    full.prefill(prompt)
+    small.prefill(prompt)
+    for t in range(3):
+        full.step(prompt[:, t])
+        small.step(prompt[:, t])
+    a, c = full.caches[0], small.caches[0]  # the first layer's keys and values depend on the tokens alone
+    for exact, rows, scale in ((a.k, c.k, c.k_scale), (a.v, c.v, c.v_scale)):
+        per_row = scale.repeat_interleave(BLOCK, dim=2)[:, :, :96, None]
+        held = rows.float() * per_row
+        # one rounding: half a step of a 4-bit mantissa (2**-4 of the value) or of e4m3's least step, 2**-10 of the
+        # scale; the block that fills row by row may be rounded again whenever its scale doubles, each time by half
+        # as much as the scale then allows: together twice that. fp32 rotation order adds under 2**-20.
+        limit = 2 * torch.maximum(exact.abs() * 2.0**-4, per_row * 2.0**-10) + 2.0**-20
+        assert ((held - exact).abs()[:, :, :48] <= limit[:, :, :48]).all()
+        assert (rows.float()[:, :, 48:] == 0).all()
+
+
+def test_decoder_with_an_8_bit_cache_does_not_care_how_a_prompt_is_cut() -> None:
+    _, whole = _decoders(1, 96)
+    _, parts = _decoders(1, 96)
+    prompt = torch.randint(0, 512, (1, 80), generator=torch.Generator().manual_seed(2))
+    want = whole.prefill(prompt)
+    for lo in (0, 32, 64):  # whole blocks: the scales are found from the same rows
+        got = parts.prefill(prompt[:, lo : lo + 32])
+    # the same cache bytes; the fp32 sums run over other shapes
+    torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-4)
+    for a, c in zip(whole.caches, parts.caches, strict=True):
+        assert (a.k.view(torch.uint8) == c.k.view(torch.uint8)).float().mean() > 0.99
+    before = [c.k.clone() for c in parts.caches]
+    parts.reset()
+    again = parts.prefill(prompt)
+    torch.testing.assert_close(again, want, rtol=1e-4, atol=1e-4)
+    assert len(before) == len(parts.caches)
+
+
+def test_decoder_refuses_other_cache_types_and_overflow() -> None:
+    from priml_b200.inference import CacheState, Decoder, Fp8KVCache
+    from priml_b200.models.presets import tiny_lm
+
+    model = tiny_lm().make().eval()
+    with pytest.raises(ValueError, match="kv_dtype"):
+        Decoder(model, batch=1, max_seq=8, kv_dtype=torch.float16)
+    dec = Decoder(model, batch=1, max_seq=8, kv_dtype=torch.float8_e4m3fn)
+    dec.prefill(torch.zeros(1, 8, dtype=torch.long))
+    with pytest.raises(ValueError, match="overflow"):
+        dec.step(torch.zeros(1, dtype=torch.long))
+    with pytest.raises(ValueError, match="positions"):
+        Fp8KVCache.alloc(CacheState.create(1, 64), heads=1, channels_head=8, cos=torch.ones(63, 4), sin=torch.ones(63, 4))
+    cache = dec.caches[0]
+    factors = torch.ones(1, 1, 16)
+    with pytest.raises(ValueError, match="cos_sin"):
+        model.blocks[0].attn(torch.zeros(1, 1, 128), cache=cache, cos_sin=(factors, factors))

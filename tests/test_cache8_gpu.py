@@ -342,3 +342,32 @@ def test_refusals_on_the_device() -> None:
     with pytest.raises(ValueError, match="overlap"):
         ops.rotary_append(q, x, x, k, v, ks, vs[:, :1].expand(-1, 2, -1), n)
     assert ops.cache_attention(q, k[:1].expand(2, -1, -1, -1), v, ks, vs, n).shape == q.shape  # reading one is fine
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_decoder_with_an_8_bit_cache_graph_equals_eager(head_dim: int) -> None:
+    from priml_b200.inference import Decoder
+    from priml_b200.models.presets import dense_lm
+
+    torch.manual_seed(0)
+    cfg = dense_lm(vocab=512, d_model=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=head_dim, ffn_hidden=512,
+                   rope_theta=1e4, norm_eps=1e-6, init_std=None)  # fmt: skip
+    model = cfg.make().cuda().to(torch.bfloat16).eval()
+    prompt = torch.randint(0, 512, (4, 33), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    kw = dict(batch=4, max_seq=128, kv_dtype=torch.float8_e4m3fn)
+    graphed, eager = Decoder(model, **kw), Decoder(model, **kw, cuda_graph=False)
+    assert torch.equal(
+        graphed.generate(prompt, max_new_tokens=40, temperature=0), eager.generate(prompt, max_new_tokens=40, temperature=0)
+    )
+    for a, c in zip(graphed.caches, eager.caches, strict=True):
+        assert torch.equal(a.k.float()[:, :, :72], c.k.float()[:, :, :72]) and torch.equal(a.v_scale, c.v_scale)
+    exact = Decoder(model, batch=4, max_seq=128, cuda_graph=False)
+    exact.prefill(prompt)
+    eager.reset()
+    eager.prefill(prompt)
+    k, c = exact.caches[0].k[:, :, :33].float(), eager.caches[0]
+    scale = c.k_scale.repeat_interleave(32, dim=2)[:, :, :33, None]
+    # the bf16 cache's keys are rounded by 2**-9 of themselves, the 8-bit ones by 2**-4 or by 2**-10 of the scale
+    limit = torch.maximum(k.abs() * (2.0**-4 + 2.0**-8), scale * 2.0**-10 + k.abs() * 2.0**-8) + 2.0**-20
+    assert ((c.k.float()[:, :, :33] * scale - k).abs() <= limit).all()
+    _status_clean()
