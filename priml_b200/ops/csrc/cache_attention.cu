@@ -18,11 +18,11 @@
 //   O^T = V^T P^T  A: V^T.  A lane holds 16 (D = 64: 8) consecutive channels of 4 keys; bytes of
 //                  neighbouring keys are interleaved (prmt) into the k-pairs of the fragment.
 //                  B: P^T from S^T by an 8 x 8 transpose (movmatrix).
-// One scale belongs to one 32-key step, so K's scale multiplies the scores and V's the step's own
-// accumulator, which is then added to the running one (the same multiply-add carries the
-// softmax's rescaling). Query rows are normalised by a power of two to fit f16 (exact; the factor
-// goes to the scores). P is rounded to f16 as 2^10 p: half a step is 2^-11 relative down to
-// p = 2^-24, less than bf16's 2^-9 of the output, and far tails stay above zero.
+// One scale belongs to one 32-key step: K's multiplies the scores; V's goes into the weights,
+// w = 2^(s + ev - m), m the running maximum of s + ev, while the row sum adds w 2^-ev. So the weights
+// fit f16 whatever the scales. Query rows are normalised by a power of two to fit f16 (exact; the
+// factor goes to the scores). Weights are rounded to f16 as 2^10 w: half a step is 2^-11 relative down
+// to w = 2^-24, less than bf16's 2^-9 of the output, and far tails stay above zero.
 //
 // Work split: the key blocks of all (sequence, KV head, row group) items form one list, cut into
 // equal runs over the grid on the device from the lengths, so ragged batches load all SMs alike
@@ -355,30 +355,57 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
               if (key > kmax[rt][e & 1] || key < kmin[rt][e & 1]) s[rt][mt][e] = -INFINITY;
             }
       }
-      // ------------------------------------------ running maximum, P
-      uint32_t pf[RT][2][2];
-      float corr[RT][2];
+      // ------------------------------------------ weights 2^(s + ev - m + 10)
+      // m follows the maximum of s + ev when that has grown by 2^4: weights stay under 2^14, and most
+      // steps need no exchange between lanes and leave O as it is.
+      const float ev = __log2f(vs_now), vi = 1.f / vs_now;
+      bool grow = false;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float f = rf[rt][e] * ks_now;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            // a hidden key stays -inf whatever the factor's sign or size
             float& x0 = s[rt][mt][e];
             float& x1 = s[rt][mt][e + 2];
-            x0 = x0 == -INFINITY ? x0 : x0 * f;
-            x1 = x1 == -INFINITY ? x1 : x1 * f;
+            if (edge) {  // a hidden key stays -inf whatever the factor's sign or size
+              x0 = x0 == -INFINITY ? x0 : fmaf(x0, f, ev);
+              x1 = x1 == -INFINITY ? x1 : fmaf(x1, f, ev);
+            } else {
+              x0 = fmaf(x0, f, ev);
+              x1 = fmaf(x1, f, ev);
+            }
           }
-          float mx = fmaxf(fmaxf(s[rt][0][e], s[rt][0][e + 2]), fmaxf(s[rt][1][e], s[rt][1][e + 2]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = fmaxf(m[rt][e], mx);
-          corr[rt][e] = m[rt][e] == -INFINITY ? 0.f : exp2_fast(m[rt][e] - mn);
-          m[rt][e] = mn;
-          const float ref = mn == -INFINITY ? 0.f : mn - 10.f;
+          grow |= fmaxf(fmaxf(s[rt][0][e], s[rt][0][e + 2]), fmaxf(s[rt][1][e], s[rt][1][e + 2])) > m[rt][e] + 4.f;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float corr[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(s[rt][0][e], s[rt][0][e + 2]), fmaxf(s[rt][1][e], s[rt][1][e + 2]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = mx > m[rt][e] + 4.f ? mx : m[rt][e];
+            corr[e] = m[rt][e] == mn ? 1.f : (m[rt][e] == -INFINITY ? 0.f : exp2_fast(m[rt][e] - mn));
+            m[rt][e] = mn;
+            l[rt][e] *= corr[e];
+          }
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[rt][mt][e] *= corr[e & 1];
+        }
+      }
+      uint32_t pf[RT][2][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float ref = m[rt][e] == -INFINITY ? 0.f : m[rt][e] - 10.f;
           float add = 0.f;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
@@ -388,7 +415,7 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
               s[rt][mt][e + hh] = x;
               add += x;
             }
-          l[rt][e] = l[rt][e] * corr[rt][e] + add;
+          l[rt][e] = fmaf(add, vi, l[rt][e]);
         }
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
@@ -399,37 +426,22 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
       // ------------------------------------------ O^T += V^T P^T, two m-tiles of channels per word
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
-        float c[RT][2][4];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[rt][x][e] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const uint32_t r0 = st.v[4 * ks][w], r1 = st.v[4 * ks + 1][w], r2 = st.v[4 * ks + 2][w],
-                         r3 = st.v[4 * ks + 3][w];
+          const uint32_t r0 = st.v[4 * ks][w], r1 = st.v[4 * ks + 1][w], r2 = st.v[4 * ks + 2][w], r3 = st.v[4 * ks + 3][w];
           const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
           const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
           {
             const uint32_t a0 = f16x2_of(lo01), a1 = f16x2_of(lo01 >> 16), a2 = f16x2_of(lo23), a3 = f16x2_of(lo23 >> 16);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) mma_f16(c[rt][0], a0, a1, a2, a3, pf[rt][ks][0], pf[rt][ks][1]);
+            for (int rt = 0; rt < RT; ++rt) mma_f16(o[rt][2 * w], a0, a1, a2, a3, pf[rt][ks][0], pf[rt][ks][1]);
           }
           {
             const uint32_t a0 = f16x2_of(hi01), a1 = f16x2_of(hi01 >> 16), a2 = f16x2_of(hi23), a3 = f16x2_of(hi23 >> 16);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) mma_f16(c[rt][1], a0, a1, a2, a3, pf[rt][ks][0], pf[rt][ks][1]);
+            for (int rt = 0; rt < RT; ++rt) mma_f16(o[rt][2 * w + 1], a0, a1, a2, a3, pf[rt][ks][0], pf[rt][ks][1]);
           }
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              o[rt][2 * w + x][e] = fmaf(o[rt][2 * w + x][e], corr[rt][e & 1], c[rt][x][e] * vs_now);
       }
       if (more) load_v<D, RT>(st, vp, next_row, n, g, t);
     }
