@@ -46,7 +46,6 @@ constexpr int kLaunch = 640;  // whole warpgroups, so that the register split be
 // Registers per thread after the split; 640 threads are launched with 96 each.
 constexpr int kRegsSoftmax = 136, kRegsConvert = 72, kRegsIssue = 64;
 static_assert(256 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsIssue <= kLaunch * 96, "register split");
-constexpr int kGroupBarrier = 1;  // named barrier of the softmax warps
 constexpr float kShift = 7.f;     // weights are up to 2^(threshold + shift) = 2^15, within f16
 constexpr int kItemCost = 3;       // an item's start and end cost a CTA about as much as this many key tiles
 constexpr int kPolyOf4 = 1;       // of four pairs of weights this one takes exp2_poly
@@ -299,7 +298,8 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
   uint64_t* q_full = o_final + 2;               // eight softmax warps
   uint64_t* piece_full = q_full + 1;            // [kPieces]
   uint64_t* piece_empty = piece_full + kPieces; // [kPieces] softmax, converting and MMA warps
-  uint64_t* drain = piece_empty + kPieces;
+  uint64_t* group_bar = piece_empty + kPieces;  // the softmax warps
+  uint64_t* drain = group_bar + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ long long warp_sum[kLaunch / 32];
@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
       mbar_init(&piece_full[s], 1);
       mbar_init(&piece_empty[s], kSoftmaxWarps + 2 * kConvertWarps + 2);
     }
+    mbar_init(group_bar, kSoftmaxWarps);
     mbar_init(drain, 2);
     *abort_flag = 0;
     fence_barrier_init();
@@ -390,9 +391,14 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + t * kKeys + lane_off;
     const uint32_t tO = tmem + 2 * kKeys + t * D + lane_off;
-    uint32_t tiles_before = 0, n_seg = 0;
+    uint32_t tiles_before = 0, n_seg = 0, meetings = 0;
     uint32_t s_phase = 0, n_pv = 0;  // parity of each score buffer's next fill; steps so far
     bool ok = true;
+    auto meet = [&]() {  // all softmax warps, with a limit (a named barrier would wait for a warp that gave up)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(group_bar);
+      ok = mbar_wait_warp(group_bar, meetings++ & 1, p.status, kTimeoutEpilogue, abort_flag) && ok;
+    };
     for (; ok; ++n_seg) {
       if (!(ok = mbar_wait_warp(&piece_full[n_seg % kPieces], (n_seg / kPieces) & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
       const Piece& x = pieces[n_seg % kPieces];
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           scratch[0] = m;
           scratch[1] = l;
         }
-        asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
+        meet();
         if (t == 0) {
           const float m2 = scratch[0], l2 = scratch[1];
           const float mm = fmaxf(m, m2);
@@ -574,7 +580,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           l = l * f_own + l2 * f_other;
           m = mm;
         }
-        asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
+        meet();
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       float* part = p.part + ((2LL * blockIdx.x + x.begins) * kCacheTcRows + (both ? r : t * 128 + r)) * (D + 2);
@@ -598,8 +604,8 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
             for (int i = 0; i < 8; ++i)
               *reinterpret_cast<float4*>(scratch + 4 * i) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
           }
-          asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
-          if (t == 0) {
+          meet();
+          if (t == 0 && ok) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float4 z = *reinterpret_cast<const float4*>(scratch + 4 * i);
@@ -609,7 +615,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
               y[4 * i + 3] = fmaf(z.w, f_other, y[4 * i + 3]);
             }
           }
-          asm volatile("bar.sync %0, %1;" ::"n"(kGroupBarrier), "n"(kSoftmaxWarps * 32) : "memory");
+          meet();
         }
         if (write && whole) {
           uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
@@ -624,6 +630,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           for (int i = 0; i < 16; ++i) *reinterpret_cast<float2*>(part + c * 32 + 2 * i) = make_float2(y[2 * i], y[2 * i + 1]);
         }
       }
+      if (!ok) break;
       tiles_before += count;
       tc_fence_before();
       __syncwarp();
