@@ -273,7 +273,8 @@ def rotary_append(
     ``[B, Hkv, ceil(T / 32)]``) hold one power of two per 32 rows and head, the least one with which the
     rows stay within e4m3's range: a row stands for ``row * scale``. Appending to a block that holds rows
     already keeps its scale or, for larger values, raises it and requantises those rows. Values that are
-    not finite are stored as NaN. Tokens past ``T`` are not stored. Returns the rotated q.
+    not finite are stored as NaN. Tokens past ``T`` are not stored. Returns the rotated q, or ``q`` itself
+    where nothing is rotated.
 
     On CUDA with bf16 and 64 or 128 channels a head this is one kernel (``csrc/rotary.cu``).
     """
@@ -288,6 +289,8 @@ def rotary_append(
     if cos is not None and (cos.ndim != 2 or cos.shape != sin.shape or not 2 <= 2 * cos.shape[1] <= q.shape[-1] or cos.shape[0] < 1):
         raise ValueError(f"cos and sin must be [positions, R/2] tables with 2 <= R <= {q.shape[-1]}, got {tuple(cos.shape)}.")
     _check_cache(q, k_cache, v_cache, k_scale, v_scale, lengths)
+    if k_cache.numel() and (k_cache.data_ptr() == v_cache.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr()):
+        raise ValueError("keys and values need caches and scales of their own.")
     if any(x.requires_grad for x in (q, k, v)) and torch.is_grad_enabled():
         raise RuntimeError("rotary_append has no gradient: call it under torch.no_grad().")
     return reference.rotary_append(q, k, v, k_cache, v_cache, k_scale, v_scale, lengths, cos, sin, interleave)

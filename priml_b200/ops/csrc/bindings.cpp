@@ -755,6 +755,7 @@ std::vector<Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& cos, 
   p.sign = static_cast<float>(sign);
   p.interleave = interleave;
   pb::rotary(p, st == torch::kBFloat16 ? 0 : (st == torch::kFloat32 ? 1 : 2), stream());
+  C10_CUDA_CHECK(cudaGetLastError());
   return {qo, ko};
 }
 
@@ -854,6 +855,8 @@ Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tenso
   check_cache(k_cache, k_scale, q_, B, Hkv, T, D, "k");
   check_cache(v_cache, v_scale, q_, B, Hkv, T, D, "v");
   const Tensor lengths = lengths_of(lengths_, q_, B);
+  PB_VALUE(k_cache.numel() == 0 || (k_cache.data_ptr() != v_cache.data_ptr() && k_scale.data_ptr() != v_scale.data_ptr()),
+           "keys and values need caches and scales of their own");
   check_planes(k_cache, "k cache");
   check_planes(v_cache, "v cache");
   check_planes(k_scale, "k scales");
@@ -897,6 +900,7 @@ Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tenso
   p.B = static_cast<int>(B), p.s = static_cast<int>(s), p.H = static_cast<int>(H), p.Hkv = static_cast<int>(Hkv);
   p.T = static_cast<int>(T);
   pb::rotary_append(p, static_cast<int>(D), interleave, stream());
+  C10_CUDA_CHECK(cudaGetLastError());
   return out;
 }
 
@@ -956,6 +960,7 @@ Tensor cache_attn(const Tensor& q_, const Tensor& k, const Tensor& v, const Tens
       p.plan = reinterpret_cast<long long*>(work.data_ptr<float>());
       p.part = work.data_ptr<float>() + 2 * plan_words;
       pb::cache_attn(p, static_cast<int>(D), stream());
+      C10_CUDA_CHECK(cudaGetLastError());
     }
   }
   return out;

@@ -210,6 +210,7 @@ struct Piece {
   int base;              // position of the chunk's first token
   int kt0, count;        // key tiles of this piece (count 0: the run is done)
   int edge_hi, edge_lo;  // a key tile at k0 needs masks if k0 > edge_hi or k0 < edge_lo
+  int lo_block;          // first block of 32 keys that any row of the tile sees
   int from[2], to[2];    // tiles of the piece that row tile 0 / 1 sees
   int both;              // at most 128 rows: the groups share them and take half of each tile
   int whole, begins;     // the piece is the whole item; it holds the item's first tile
@@ -264,6 +265,7 @@ struct Walk {
     x.count = j1 - j0;
     x.edge_hi = sp.pos0 - kKeys + 1;
     x.edge_lo = p.window >= 0 ? sp.pos1 - p.window : INT_MIN;
+    x.lo_block = p.window >= 0 ? max(sp.pos0 - p.window, 0) / kCacheBlock : 0;
     x.both = p.s * p.group - x.row0 <= 128;
     x.whole = j0 == 0 && j1 == sp.count;
     x.begins = j0 == 0;
@@ -659,10 +661,11 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
       // lanes 0-3 of the first V warp bring K's scales of the tile's blocks, lanes 4-7 V's
       const bool brings = is_v && c < 8;
       const float* scale = c < 4 ? p.k_scale + x.b * p.ks_sb + x.hk * p.ks_sh : p.v_scale + x.b * p.vs_sb + x.hk * p.vs_sh;
-      const int blocks = (n_keys + kCacheBlock - 1) / kCacheBlock;
+      // (blocks of the tile that no row sees may hold anything: their scales are not read)
+      const int blocks = (n_keys + kCacheBlock - 1) / kCacheBlock, lo_block = x.lo_block;
       auto scale_at = [&](int k0) {
         const int blk = k0 / kCacheBlock + (c & 3);
-        return brings && blk < blocks ? scale[blk] : 1.f;
+        return brings && blk >= lo_block && blk < blocks ? scale[blk] : 1.f;
       };
       int k0 = x.kt0 * kKeys;
       uint4 raw[NP];

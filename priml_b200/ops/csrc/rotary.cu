@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(kThreads, 7) rotary_append_kernel(AppendParams
   const int start = p.lengths[b];                      // first appended row
   if (start < 0 || start >= p.T) return;
   const int end = static_cast<int>(min(static_cast<long long>(start) + p.s, static_cast<long long>(p.T)));
+  if (start / kRows + static_cast<long long>(nth) > (end - 1) / kRows) return;
   const int cb = start / kRows + nth;                  // cache block
   const int row0 = cb * kRows;
   const int lo = max(start - row0, 0);                 // appended rows of the block: [lo, hi)

@@ -147,6 +147,50 @@ def test_attention_of_more_sequences_than_one_launch_takes() -> None:
     assert (out.cpu().double() - want).abs().max().item() <= attention_tolerance(v, vs)
 
 
+@pytest.mark.parametrize("s", [1, 4, 30])
+def test_scales_of_blocks_that_no_query_sees_may_hold_anything(s: int) -> None:
+    from priml_b200 import ops
+
+    b, h, hkv, t, d, window = 2, 4, 1, 500, 64, 50
+    k, ks = filled_cache(b, hkv, t, d, seed=1, device="cuda")
+    v, vs = filled_cache(b, hkv, t, d, seed=2, device="cuda")
+    q = (torch.randn(b, s, h, d, generator=torch.Generator().manual_seed(s)) * 0.125).bfloat16().cuda()
+    ends = [430, 300]
+    n = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    clean = ops.cache_attention(q, k, v, ks, vs, n, window=window)
+    for i, end in enumerate(ends):
+        lo, hi = (end - s - window) // 32, -(-end // 32)
+        for scale in (ks, vs):
+            scale[i, :, :lo], scale[i, :, hi:] = float("nan"), float("inf")
+        for rows in (k, v):
+            rows.view(torch.uint8)[i, :, : end - s - window] = 0x7F
+    assert torch.equal(ops.cache_attention(q, k, v, ks, vs, n, window=window), clean)
+
+
+def test_many_row_launches_are_split_by_sequences_and_by_tokens() -> None:
+    from priml_b200 import ops
+
+    b, s = 1100, 20  # more row tiles than one launch lists
+    k, ks = filled_cache(b, 1, 40, 64, seed=3, device="cuda")
+    v, vs = filled_cache(b, 1, 40, 64, seed=4, device="cuda")
+    ends = [20 + (7 * i) % 21 for i in range(b)]
+    q = (torch.randn(b, s, 1, 64, generator=torch.Generator().manual_seed(1)) * 0.125).bfloat16().cuda()
+    out = ops.cache_attention(q, k, v, ks, vs, torch.tensor(ends, dtype=torch.int32, device="cuda"))
+    pick = [0, 1, 1022, 1023, 1024, 1025, 1099]
+    want = attend64(q[pick], k[pick], v[pick], ks[pick], vs[pick], [ends[i] for i in pick])
+    assert (out[pick].cpu().double() - want).abs().max().item() <= attention_tolerance(v, vs)
+
+    s, h, t = 600, 512, 640  # 512 query heads on one KV head: 1200 row tiles of one sequence
+    k, ks = filled_cache(1, 1, t, 64, seed=5, device="cuda")
+    v, vs = filled_cache(1, 1, t, 64, seed=6, device="cuda")
+    q = (torch.randn(1, s, h, 64, generator=torch.Generator().manual_seed(2)) * 0.125).bfloat16().cuda()
+    out = ops.cache_attention(q, k, v, ks, vs, torch.tensor([630], dtype=torch.int32, device="cuda"))
+    for i in (0, 1, 511, 512, 513, 599):  # query i alone stands at 30 + i
+        want = attend64(q[:, i : i + 1], k, v, ks, vs, [31 + i])
+        assert (out[:, i : i + 1].cpu().double() - want).abs().max().item() <= attention_tolerance(v, vs)
+    _status_clean()
+
+
 def test_long_cache_past_32_bit_offsets() -> None:
     """Byte offsets past 2**31 inside one cache: 2 sequences x 2 heads x 2**23 + 40 rows of 128."""
     from priml_b200 import ops
@@ -264,6 +308,21 @@ def test_rotary_and_its_gradient_match_torch(b, s, h, hk, d, rot, per_seq, dtype
         assert a.dtype == dtype and torch.equal(a, c)
 
 
+@pytest.mark.parametrize("shape", [(1, 6, 1, 8), (6, 4, 8), (2, 6, 4, 8)])  # one table as a batch, factors per head
+def test_rotary_broadcasts_its_factors(shape: tuple) -> None:
+    from priml_b200 import ops
+    from priml_b200.models.rope import RoPE
+    from priml_b200.ops import reference
+
+    q, k = torch.randn(2, 6, 4, 24, device="cuda"), torch.randn(2, 6, 4, 24, device="cuda")
+    ang = torch.randn(shape, device="cuda")
+    got = ops.rotary(q, k, ang.cos(), ang.sin(), interleave=True)
+    assert torch.equal(got[0], reference.rotate(q, ang.cos(), ang.sin(), True))
+    assert torch.equal(RoPE.rotate(q, k, ang.cos(), ang.sin(), True)[1], reference.rotate(k, ang.cos(), ang.sin(), True))
+    learned = ang.cos().requires_grad_()  # factors with a gradient take the torch operations
+    assert torch.autograd.grad(ops.rotary(q, k, learned, ang.sin(), interleave=True)[0].sum(), learned)[0].shape == shape
+
+
 def test_rotary_second_derivative_and_one_sided_gradients() -> None:
     from priml_b200 import ops
 
@@ -341,6 +400,12 @@ def test_refusals_on_the_device() -> None:
         ops.rotary_append(q, x, x, k[:1].expand(2, -1, -1, -1), v, ks, vs, n)
     with pytest.raises(ValueError, match="overlap"):
         ops.rotary_append(q, x, x, k, v, ks, vs[:, :1].expand(-1, 2, -1), n)
+    with pytest.raises(ValueError, match="of their own"):
+        ops.rotary_append(q, x, x, k, k, ks, vs, n)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.cache_attention(q.detach().requires_grad_(), k, v, ks, vs, n)
+    with pytest.raises(ValueError):
+        ops.rotary_append(q, x, x, k, v, ks, vs, n, cos=torch.ones(4, 33, device="cuda"), sin=torch.ones(4, 33, device="cuda"))
     assert ops.cache_attention(q, k[:1].expand(2, -1, -1, -1), v, ks, vs, n).shape == q.shape  # reading one is fine
 
 
