@@ -760,8 +760,8 @@ std::vector<Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& cos, 
 }
 
 // The rotation with its gradient, the rotation by -sin (which is differentiable in turn). The autograd node
-// is C++: a training step makes one per attention layer and direction, and a Python node costs more host
-// time (about 45 us for a forward and backward, against 15 us) than the kernels take at most sizes.
+// is C++: a training step makes one per attention layer, and at small sizes its host time is what counts (a
+// forward and backward of a few tokens, torch's own engine included: 110 us with a Python node, 80 us with this).
 class RotaryFn : public torch::autograd::Function<RotaryFn> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,

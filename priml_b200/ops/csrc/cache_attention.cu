@@ -9,9 +9,23 @@
 // Per SM that is about 23 cached values per clock, each needing `group` multiply-adds and a
 // conversion, which the fp32 pipes cannot do at group 4 and up. So the products run on the
 // tensor cores as m16n8k16 f16 products with keys (then channels) on M and query rows on N: the
-// e4m3 operand converts exactly to f16 in registers, straight from 16-byte global loads, with no
-// shared memory in between. tcgen05 would need the converted tile in shared memory and 128 rows
-// of M per product; here N = 8 rows are useful and the pipes idle anyway.
+// e4m3 operand converts exactly to f16 in registers. tcgen05 would need the converted tile in shared
+// memory and 128 rows of M per product; here 8 or 16 rows are useful and the pipes idle anyway. Each warp
+// copies its own 32-key steps (cp.async, two or three steps ahead), so no barrier of the CTA stands between
+// the memory and the products.
+//
+// Measured (B200, 32 query and 8 KV heads): 64 sequences of 8192 tokens, heads of 128, 1.08 GB, in 175 us,
+// 6.15 TB/s (a plain copy: 6.5), while the SMs run at 1965 MHz, and 193 us once the power cap has them at 1700;
+// one sequence of 1000 tokens, heads of 64, 14 us, of which the kernels take 8. What is left is the latency of
+// a 32-key step that three CTAs per SM do not quite hide. Other forms: the bytes loaded straight into
+// registers 196 us and, at 16 rows, 41 us where this takes 38.6 (nine sequences of 1 to 100001 tokens); a
+// ring whose lanes copy only what they read themselves (half lines of K) 240 us when direct loads took 214;
+// four CTAs per SM 226 us (registers spill); a second wave of short runs for the SMs that finish first (equal
+// runs end 25 % apart) 208 us, its CTAs' starts costing more than they even out.
+//
+// Up to 16 rows per KV head come here, in one or two tiles of 8; more go to the tensor-memory form
+// (cache_attention_tc.cu). Both sides, 20 rows per KV head, 8 sequences of up to 16384 tokens: two passes
+// over the cache here 134 us, four tiles in one pass 118 us (255 registers and spills), there 70 us.
 //
 //   S^T = K Q^T    A: K rows (lane g holds rows g, g + 8), B: Q.  The contraction index d is
 //                  permuted so that a lane's 16 consecutive bytes of a row are four k-steps.
@@ -43,7 +57,9 @@ using namespace cache8;
 
 constexpr int kWarps = 4;
 constexpr int kMaxSeqs = 1024;  // sequences per launch (prefix table in shared memory)
-constexpr int kItemCost = 4;    // an item's start and end cost a CTA about as much as this many key blocks
+// An item's start and end cost a CTA about as much as this many key blocks (nine sequences of 1 to 100001
+// tokens: 43 us without it, 39 with it).
+constexpr int kItemCost = 4;
 constexpr int kMinRun = kItemCost + 4;  // list entries per CTA at least: an item's cost and a block per warp
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -73,56 +89,90 @@ __device__ __forceinline__ int seq_blocks(const CacheAttnParams& p, int b, long 
   return static_cast<int>((n + kCacheBlock - 1) / kCacheBlock) - first;
 }
 
+// Shared memory of a CTA: per warp a ring of kStages 32-key steps: K rows, V rows, the step's two scales.
+// Copies take whole 128-byte lines; a row's 16-byte chunks are permuted so that the fragment reads below
+// meet no bank twice. The warps' results are merged over the ring's memory at an item's end.
 template <int D, int RT>
-struct Step {  // one warp's raw bytes of a 32-key step
-  static constexpr int KV = D / 64;  // 16-byte K pieces per row half... (16 bytes at hf * 64 + t * 16)
-  uint4 k[4][KV];                    // rows g, g + 8, g + 16, g + 24
-  uint32_t v[8][D / 32];             // keys 2t, 2t+1, 2t+8, 2t+9 (+16); D / 8 bytes at g * D / 8
-  float ks, vs;
+struct Cfg {
+  static constexpr int kStages = D == 128 && RT == 1 ? 2 : 3;
+  static constexpr int kRows = kCacheBlock * D;      // bytes of K or V in a step
+  static constexpr int kStage = 2 * kRows + 16;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kRed = kWarps * RT * 8 * (D + 2) * 4;
+  static constexpr int kBytes = kRing > kRed ? kRing : kRed;
+  static constexpr int kCtas = RT == 1 ? 3 : 2;      // per SM, what the registers allow
 };
 
-template <int D, int RT>
-__device__ __forceinline__ void load_k(Step<D, RT>& st, const uint8_t* k, int base, int n, int g, int t) {
+// Where chunk c (16 bytes) of row r of a step lies. D = 128: c ^ (r & 7) within the row; D = 64: two rows
+// make a line of eight chunks, and the line's number moves them by pairs.
+template <int D>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+  return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (((r >> 1) & 3) << 1)) << 4);
+}
+// The key (of eight) that row g of an S^T tile stands for. At D = 128 rows 2i and 2i + 1 have to differ in
+// bit 2 for K's reads, and rows 2t (and 2t + 1) in their upper bits for V's: 0 5 2 7 4 1 6 3.
+template <int D>
+__device__ __forceinline__ int key_of(int g) {
+  return D == 128 ? (g & 1 ? (g + 4) & 7 : g) : g;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t* src, bool real) {
+  const int n = real ? BYTES : 0;  // the rest is zero-filled
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Starts the copies of the step at key row `base` (keys past n are zero-filled).
+template <int D>
+__device__ __forceinline__ void start_step(uint32_t stage, const uint8_t* k, const uint8_t* v, const float* ks,
+                                           const float* vs, int base, int n, int lane) {
+  constexpr int PR = D / 16;  // chunks per row
+  const int c = lane % PR, r0 = lane / PR;
+  const long long off = static_cast<long long>(base) * D + lane * 16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = base + i * 8 + g;
-#pragma unroll
-    for (int hf = 0; hf < D / 64; ++hf)
-      st.k[i][hf] = row < n ? load16(k + static_cast<long long>(row) * D + hf * 64 + t * 16) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < PR; ++i) {
+    const int r = r0 + i * (32 / PR);
+    const bool real = base + r < n;
+    const uint32_t dst = stage + chunk_at<D>(r, c);
+    copy_async<16>(dst, k + (real ? off + i * 512 : 0), real);
+    copy_async<16>(dst + kCacheBlock * D, v + (real ? off + i * 512 : 0), real);
   }
+  if (lane < 2)
+    copy_async<4>(stage + 2 * kCacheBlock * D + 4 * lane,
+                  reinterpret_cast<const uint8_t*>((lane ? vs : ks) + base / kCacheBlock), true);
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
 }
 
 template <int D, int RT>
-__device__ __forceinline__ void load_v(Step<D, RT>& st, const uint8_t* v, int base, int n, int g, int t) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = base + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + 2 * t + (i & 1);
-    const uint8_t* at = v + static_cast<long long>(row) * D + g * (D / 8);
-    if (D == 128) {
-      const uint4 r = row < n ? load16(at) : make_uint4(0, 0, 0, 0);
-      st.v[i][0] = r.x;
-      st.v[i][1] = r.y;
-      st.v[i][D / 32 - 2] = r.z;
-      st.v[i][D / 32 - 1] = r.w;
-    } else {
-      uint2 r = make_uint2(0, 0);
-      if (row < n)
-        asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(at));
-      st.v[i][0] = r.x;
-      st.v[i][1] = r.y;
-    }
-  }
-}
-
-template <int D, int RT>
-__global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_kernel(const CacheAttnParams p) {
   constexpr int R = RT * 8;         // query rows per item
   constexpr int KS = D / 16;        // k-steps of the score product = m-tiles of the value product
   __shared__ long long prefix[kMaxSeqs + 1];
   __shared__ long long warp_sum[kWarps];
-  __shared__ float red[kWarps][R][D + 2];
+  using C = Cfg<D, RT>;
+  extern __shared__ __align__(16) uint8_t ring_smem[];
+  float(*red)[R][D + 2] = reinterpret_cast<float(*)[R][D + 2]>(ring_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(ring_smem) + warp * C::kStages * C::kStage;
 
   // ------------------------------------------------ the block list: prefix per sequence, this CTA's run
   const long long heads = p.mult;  // (KV head, row group) items per sequence
@@ -277,20 +327,21 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
         for (int e = 0; e < 4; ++e) o[rt][mt][e] = 0.f;
     }
 
-    Step<D, RT> st;
-    int j = j0 + warp;
-    if (j < j1) {
-      const int base_row = (first + j) * kCacheBlock;
-      st.ks = ksp[first + j];
-      st.vs = vsp[first + j];
-      load_k<D, RT>(st, kp, base_row, n, g, t);
-      load_v<D, RT>(st, vp, base_row, n, g, t);
+#pragma unroll
+    for (int i = 0; i < C::kStages; ++i) {
+      const int ji = j0 + warp + i * kWarps;
+      if (ji < j1) start_step<D>(ring + i * C::kStage, kp, vp, ksp, vsp, (first + ji) * kCacheBlock, n, lane);
+      copy_commit();
     }
-    for (; j < j1; j += kWarps) {
+    int slot = 0;
+    for (int j = j0 + warp; j < j1; j += kWarps) {
       const int base_row = (first + j) * kCacheBlock;
-      const bool more = j + kWarps < j1;
-      const int next_row = base_row + kWarps * kCacheBlock;
-      const float ks_now = st.ks, vs_now = st.vs;
+      const uint32_t stage = ring + slot * C::kStage;
+      slot = slot + 1 == C::kStages ? 0 : slot + 1;
+      copy_wait<C::kStages - 1>();
+      __syncwarp();  // every lane's copies are there for all
+      float ks_now, vs_now;
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks_now), "=f"(vs_now) : "r"(stage + 2 * C::kRows) : "memory");
       // ------------------------------------------ S^T = K Q^T
       float s[RT][2][4];
 #pragma unroll
@@ -303,7 +354,8 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf) {
-          const uint4 ra = st.k[2 * mt][hf], rb = st.k[2 * mt + 1][hf];
+          const int r = mt * 16 + key_of<D>(g);
+          const uint4 ra = lds16(stage + chunk_at<D>(r, hf * 4 + t)), rb = lds16(stage + chunk_at<D>(r + 8, hf * 4 + t));
           const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -314,23 +366,35 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
           }
         }
       }
-      if (more) {
-        st.ks = ksp[first + j + kWarps];
-        st.vs = vsp[first + j + kWarps];
-        load_k<D, RT>(st, kp, next_row, n, g, t);
+      uint32_t vr[8][D / 32];  // keys of S^T's rows 2t, 2t+1, 2t+8, 2t+9 (+16); D / 8 bytes at channel g * D / 8
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = (i >> 2) * 16 + ((i >> 1) & 1) * 8 + key_of<D>(2 * t + (i & 1));
+        const uint32_t at = stage + C::kRows + (D == 128 ? chunk_at<D>(r, g) : chunk_at<D>(r, g >> 1) + (g & 1) * 8);
+        if (D == 128) {
+          const uint4 r = lds16(at);
+          vr[i][0] = r.x;
+          vr[i][1] = r.y;
+          vr[i][D / 32 - 2] = r.z;
+          vr[i][D / 32 - 1] = r.w;
+        } else {
+          const uint2 r = lds8(at);
+          vr[i][0] = r.x;
+          vr[i][1] = r.y;
+        }
       }
       const bool edge = base_row + kCacheBlock - 1 > lo_max || base_row < hi_min;
       if (edge) {
         // A value row may hold NaN where only some rows see it: its bytes become zero, and the
         // scores of the rows that do see it become NaN.
-        uint32_t bad = 0;  // bit i: key i of st.v has a NaN in this lane's channels
+        uint32_t bad = 0;  // bit i: key i of vr has a NaN in this lane's channels
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           uint32_t any = 0;
 #pragma unroll
           for (int w = 0; w < D / 32; ++w) {
-            const uint32_t nb8 = nan_bytes(st.v[i][w]);
-            st.v[i][w] &= ~nb8;
+            const uint32_t nb8 = nan_bytes(vr[i][w]);
+            vr[i][w] &= ~nb8;
             any |= nb8;
           }
           bad |= any != 0 ? 1u << i : 0u;
@@ -340,7 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
           uint32_t mine = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (bad >> i & 1) mine |= 1u << ((i >> 2) * 16 + ((i >> 1) & 1) * 8 + 2 * t + (i & 1));
+            if (bad >> i & 1) mine |= 1u << ((i >> 2) * 16 + ((i >> 1) & 1) * 8 + key_of<D>(2 * t + (i & 1)));
           badrows = __reduce_or_sync(0xffffffffu, mine);
         }
 #pragma unroll
@@ -349,7 +413,7 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int in = mt * 16 + (e >> 1) * 8 + g;
+              const int in = mt * 16 + (e >> 1) * 8 + key_of<D>(g);
               const int key = base_row + in;
               if (badrows >> in & 1) s[rt][mt][e] = NAN;
               if (key > kmax[rt][e & 1] || key < kmin[rt][e & 1]) s[rt][mt][e] = -INFINITY;
@@ -428,7 +492,7 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
       for (int w = 0; w < D / 32; ++w) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const uint32_t r0 = st.v[4 * ks][w], r1 = st.v[4 * ks + 1][w], r2 = st.v[4 * ks + 2][w], r3 = st.v[4 * ks + 3][w];
+          const uint32_t r0 = vr[4 * ks][w], r1 = vr[4 * ks + 1][w], r2 = vr[4 * ks + 2][w], r3 = vr[4 * ks + 3][w];
           const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
           const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
           {
@@ -443,10 +507,15 @@ __global__ void __launch_bounds__(kWarps * 32, RT == 1 ? 3 : 2) cache_attn_kerne
           }
         }
       }
-      if (more) load_v<D, RT>(st, vp, next_row, n, g, t);
+      __syncwarp();  // every lane has read the stage
+      if (j + C::kStages * kWarps < j1)
+        start_step<D>(stage, kp, vp, ksp, vsp, base_row + C::kStages * kWarps * kCacheBlock, n, lane);
+      copy_commit();
     }
 
-    // ---------------------------------------------- merge the warps
+    // ---------------------------------------------- merge the warps (over the ring: all copies have landed)
+    copy_wait<0>();
+    __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -587,11 +656,18 @@ template <int D, int RT>
 int ctas_per_sm() {
   static int cached = 0;
   if (cached == 0) {
+    cudaFuncSetAttribute(cache_attn_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, RT>::kBytes);
     int n = 0;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_attn_kernel<D, RT>, kWarps * 32, 0);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_attn_kernel<D, RT>, kWarps * 32, Cfg<D, RT>::kBytes);
     cached = n < 1 ? 1 : n;
   }
   return cached;
+}
+
+template <int D, int RT>
+void launch(const CacheAttnParams& p, cudaStream_t stream) {
+  cudaFuncSetAttribute(cache_attn_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, RT>::kBytes);
+  cache_attn_kernel<D, RT><<<p.grid, kWarps * 32, Cfg<D, RT>::kBytes, stream>>>(p);
 }
 
 int row_groups_of_8(const CacheAttnParams& p) { return p.s * p.group <= 8 ? 1 : 2; }
@@ -643,11 +719,9 @@ void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
   if (cache_attn_many_rows(p))
     cache_attn_tc(p, D, stream);
   else if (D == 64)
-    one ? cache_attn_kernel<64, 1><<<p.grid, kWarps * 32, 0, stream>>>(p)
-        : cache_attn_kernel<64, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
+    one ? launch<64, 1>(p, stream) : launch<64, 2>(p, stream);
   else
-    one ? cache_attn_kernel<128, 1><<<p.grid, kWarps * 32, 0, stream>>>(p)
-        : cache_attn_kernel<128, 2><<<p.grid, kWarps * 32, 0, stream>>>(p);
+    one ? launch<128, 1>(p, stream) : launch<128, 2>(p, stream);
   const dim3 merge(p.grid, p.item_rows < 32 ? p.item_rows : 32);
   if (D == 64)
     cache_attn_merge_kernel<64><<<merge, kMergeWarps * 32, 0, stream>>>(p);

@@ -16,7 +16,10 @@
 // keeps max(e_old, e_new); when e grows its old rows are requantised by the exact factor
 // 2^(e_old - e). Values that are not finite are stored as NaN and do not take part in amax.
 //
-// Both are bound by their bytes: each value is read and written once.
+// Both are bound by their bytes: each value is read and written once. Measured (B200, bf16):
+//   rotation  8 x 2048 tokens, 32 + 8 heads of 128, 32 turned: 335 MB in 58 us, 5.8 TB/s (a plain copy: 6.5)
+//   append    4 x 2048 tokens, 32 + 8 heads of 128: 186 MB in 53 us, 3.5 TB/s; one token for 64 sequences 9 us,
+//             which is the host's time for the call
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -296,7 +299,9 @@ __device__ __forceinline__ void widen(const Vec<__nv_bfloat16, N>& raw, float (&
 // four warps, eight rows in flight each. The rest take one (sequence, KV head, block of 32 cache rows, K
 // or V) each: pass one leaves the rows' values in registers and finds amax, pass two requantises old
 // rows if need be and stores. What bounds it is the instructions per value next to 3 bytes of traffic, so
-// values are kept in vectors and the rare case (something not finite) in a branch of its own.
+// values are kept in vectors and the rare case (something not finite) in a branch of its own. Seven blocks per
+// SM (72 registers) against the four of an unbounded build (93): more rows in flight. Blocks of 256 threads
+// were slower: the two barriers then hold up twice the rows.
 template <int D, bool INTER, bool EASY>
 __global__ void __launch_bounds__(kThreads, 7) rotary_append_kernel(AppendParams p) {
   constexpr int N = D / 32;
