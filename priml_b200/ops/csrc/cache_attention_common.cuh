@@ -23,6 +23,13 @@ __device__ __forceinline__ uint32_t f16x2_of(uint32_t two_bytes) {
   return d;
 }
 
+// The same of a word's upper two bytes.
+__device__ __forceinline__ uint32_t f16x2_of_upper(uint32_t w) {
+  uint32_t d;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\ncvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(d) : "r"(w));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);

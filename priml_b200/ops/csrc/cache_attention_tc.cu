@@ -27,10 +27,12 @@
 // next piece while the softmax warps finish the last.
 //
 // Measured (B200, D = 128): a 2048-token prompt chunk that ends a cache of 32768, 32 + 8 heads, 1.07 TFLOP in
-// 1.28 ms (830 TFLOP/s under the power cap, 950 at full clocks). The tensor cores wait for the softmax warps'
+// 1.23 ms (863 TFLOP/s under the power cap). The tensor cores wait for the softmax warps'
 // chain per 64 keys (score load, exponent, weight store), whose latency two buffers per group hide in part.
 // Sixteen softmax warps of 64 registers were slower (1.70 against 1.29 ms: the rows' state spills), as was raw
-// e4m3 staged through shared memory by bulk copies; a prefetch into L2 changed nothing (loads are a tile ahead).
+// e4m3 staged through shared memory by bulk copies. Five tokens each of 8 sequences take 69 us, bound by the
+// conversion: about 2000 clocks per tile of K or V and its four warps. Rows copied into the idle lanes of the
+// tile, each copy with a part of the keys, halve the softmax's time there and change nothing in all (70 us).
 // TMEM: S_0 [0, 64) and [64, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1; P lies over the first half
 // of its scores.
 #include "attention_common.cuh"
@@ -658,6 +660,10 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
     uint8_t* tiles = is_v ? sV : sK;
     uint64_t* full = is_v ? v_full : k_full;
     uint64_t* empty = is_v ? v_empty : k_empty;
+    // The tile behind the next one is brought into L2 where several row tiles read it (a 2048-token chunk over
+    // 32768 tokens: 1256 us without, 1228 with it); read once, it only costs the asking (five tokens each of 8
+    // sequences: 69 us without, 71 with it).
+    const bool far_ahead = p.tiles > 1 && c == 0;
     uint32_t tile_no = 0;
     bool ok = true;
     for (uint32_t seg = 0; ok; ++seg) {
@@ -719,22 +725,27 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           for (int i = half * NP / 2; i < (half + 1) * NP / 2; ++i) {
             const int row = row_c + i * (128 / PR);
             uint8_t* base = tile + (piece >> 2) * kChunkBytes + row * 128;
-            const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-            uint32_t f[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              f[2 * e] = f16x2_of(u[e]);
-              f[2 * e + 1] = f16x2_of(u[e] >> 16);
-            }
-            const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
             // the pieces of a row's two 64-channel chunks share banks: the upper chunk's lanes store
             // their halves in the other order
             const int p0 = 2 * (piece & 3);
             const bool swap = piece >= 4;
-            *reinterpret_cast<uint4*>(base + (((p0 + swap) ^ (row & 7)) << 4)) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(base + (((p0 + !swap) ^ (row & 7)) << 4)) = swap ? lo : hi;
+            const uint32_t u[4] = {swap ? raw[i].z : raw[i].x, swap ? raw[i].w : raw[i].y, swap ? raw[i].x : raw[i].z,
+                                   swap ? raw[i].y : raw[i].w};
+            uint32_t f[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f[2 * e] = f16x2_of(u[e]);
+              f[2 * e + 1] = f16x2_of_upper(u[e]);
+            }
+            *reinterpret_cast<uint4*>(base + (((p0 + swap) ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(base + (((p0 + !swap) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
           }
           if (j + 1 < count) load(half * NP / 2, (half + 1) * NP / 2, k0 + kKeys);
+          if (far_ahead && half == 0 && j + 2 < count) {
+            const int ahead = k0 + 2 * kKeys, bytes = min(kKeys, n_keys - ahead) * D;
+            if (bytes > 0)
+              asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + static_cast<long long>(ahead) * D), "r"(bytes));
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
