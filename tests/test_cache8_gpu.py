@@ -39,6 +39,9 @@ CASES = [  # B, s, H, Hkv, T, D, ends (None: full), window
     (3, 130, 4, 2, 400, 64, [400, 131, 130], None),
     (1, 257, 2, 1, 700, 128, [690], None),
     (2, 65, 7, 1, 300, 128, [300, 66], 64),
+    (16, 1, 8, 8, 2100, 64, None, None),  # long runs: the copies' ring wraps
+    (4, 2, 32, 4, 12000, 128, [12000, 11999, 11990, 1], None),  # the same at 16 rows
+    (1, 520, 2, 1, 3001, 128, [2999], None),  # several row tiles over many key tiles
 ]
 
 
