@@ -18,7 +18,7 @@
 // 6.15 TB/s (a plain copy: 6.5), while the SMs run at 1965 MHz, and 193 us once the power cap has them at 1700;
 // one sequence of 1000 tokens, heads of 64, 14 us, of which the kernels take 8. What is left is the latency of
 // a 32-key step that three CTAs per SM do not quite hide. Other forms: the bytes loaded straight into
-// registers 196 us and, at 16 rows, 41 us where this takes 38.6 (nine sequences of 1 to 100001 tokens); a
+// registers 196 us and, at 16 rows, 41 us where this took 38.6 (nine sequences of 1 to 100001 tokens); a
 // ring whose lanes copy only what they read themselves (half lines of K) 240 us when direct loads took 214;
 // four CTAs per SM 226 us (registers spill); a second wave of short runs for the SMs that finish first (equal
 // runs end 25 % apart) 208 us, its CTAs' starts costing more than they even out.
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
   float(*red)[R][D + 2] = reinterpret_cast<float(*)[R][D + 2]>(ring_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
+  let_merge_start();
   const uint32_t ring = smem_u32(ring_smem) + warp * C::kStages * C::kStage;
 
   // ------------------------------------------------ the block list: prefix per sequence, this CTA's run
@@ -591,6 +592,7 @@ __device__ __forceinline__ void store_row(const CacheAttnParams& p, const Cut& c
 template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) cache_attn_merge_kernel(const CacheAttnParams p) {
   constexpr int N = D / 32;
+  wait_for_pieces();
   const Cut cut = get_cut(p, blockIdx.x);
   if (cut.more == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -723,10 +725,12 @@ void cache_attn(const CacheAttnParams& p, int D, cudaStream_t stream) {
   else
     one ? launch<128, 1>(p, stream) : launch<128, 2>(p, stream);
   const dim3 merge(p.grid, p.item_rows < 32 ? p.item_rows : 32);
-  if (D == 64)
-    cache_attn_merge_kernel<64><<<merge, kMergeWarps * 32, 0, stream>>>(p);
-  else
-    cache_attn_merge_kernel<128><<<merge, kMergeWarps * 32, 0, stream>>>(p);
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = merge, cfg.blockDim = dim3(kMergeWarps * 32), cfg.stream = stream, cfg.attrs = &early, cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, D == 64 ? cache_attn_merge_kernel<64> : cache_attn_merge_kernel<128>, p);
 }
 
 }  // namespace pb

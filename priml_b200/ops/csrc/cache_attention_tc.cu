@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
   __shared__ Walk walk;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  let_merge_start();
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], kConvertWarps);
