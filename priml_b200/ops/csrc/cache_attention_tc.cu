@@ -59,7 +59,6 @@ constexpr float kShift = 7.f;     // weights are up to 2^(threshold + shift) = 2
 // ran long: five tokens each of 8 ragged sequences 116 us (with it 72), four windowed prompts of 1111 tokens, 576
 // items, 144 us (109).
 constexpr int kItemCost = 3;
-constexpr int kPolyOf4 = 1;       // of four pairs of weights this one takes exp2_poly (none, two: no faster)
 constexpr int kPieces = 4;        // work pieces in flight between the walking warp and the others
 constexpr int kScratchCols = 32;  // columns that the groups exchange at a time
 
@@ -132,30 +131,6 @@ __device__ __forceinline__ void tmem_read_x32x2(uint32_t taddr, uint32_t (&a)[32
         "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31])
       : "r"(taddr), "r"(taddr + 32)
       : "memory");
-}
-
-// 2^x of two values on the multiply-add pipes, for a part of the weights: the special-function units
-// bound the softmax. Range reduction to x = n + f, f in [0, 1), by adding 1.5 * 2^23 rounded down, and
-// a cubic with the least largest relative error on [0, 1) (7.5e-5, fitted here; f16 rounds by 2.4e-4).
-// Arguments below -126 give 2^-126, which f16 rounds to zero; NaN stays NaN.
-__device__ __forceinline__ void exp2_poly(uint64_t x2, float& e0, float& e1) {
-  float x0, x1;
-  f2_unpack(x2, x0, x1);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.f));
-  x2 = f2_pack(x0, x1);
-  const float magic = 12582912.f;
-  uint64_t n2, f2;
-  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(n2) : "l"(x2), "l"(f2_pack(magic, magic)));
-  f2 = f2_sub(x2, f2_sub(n2, f2_pack(magic, magic)));
-  uint64_t y2 = f2_fma(f2, f2_pack(0.07802452f, 0.07802452f), f2_pack(0.22606724f, 0.22606724f));
-  y2 = f2_fma(y2, f2, f2_pack(0.69583347f, 0.69583347f));
-  y2 = f2_fma(y2, f2, f2_pack(0.99992523f, 0.99992523f));
-  float n0, n1;
-  f2_unpack(n2, n0, n1);  // the low bits hold n; a NaN stays in y2
-  y2 = f2_mul(y2, f2_pack(__uint_as_float((__float_as_uint(n0) << 23) + 0x3f800000u),
-                          __uint_as_float((__float_as_uint(n1) << 23) + 0x3f800000u)));
-  f2_unpack(y2, e0, e1);
 }
 
 // Descriptors of 128-byte-swizzled tiles as their low words; all share the high word. The steps of a
@@ -545,15 +520,9 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), mul2, add2);
-            float e0, e1;
-            if (i % 4 == kPolyOf4) {
-              exp2_poly(x2, e0, e1);
-            } else {
-              float x0, x1;
-              f2_unpack(x2, x0, x1);
-              e0 = fast_exp2(x0);
-              e1 = fast_exp2(x1);
-            }
+            float x0, x1;
+            f2_unpack(x2, x0, x1);
+            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);  // (0 for a hidden key, in the sum as in P)
             const uint64_t e2 = f2_pack(e0, e1);
             asm("add.rn.f32x2 %0, %0, %1;" : "+l"(rs) : "l"(e2));
             pk[i] = pack_f16(e0, e1);
