@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
       // ------------------------------------------ weights 2^(s + ev - m + 10)
       // m follows the maximum of s + ev when that has grown by 2^4: weights stay under 2^14, and most
       // steps need no exchange between lanes and leave O as it is.
-      const float ev = __log2f(vs_now), vi = 1.f / vs_now;
+      const float ev = __log2f(vs_now), vi = kSumUnit / vs_now;
       bool grow = false;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -455,9 +455,10 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             const float mn = mx > m[rt][e] + 4.f ? mx : m[rt][e];
-            corr[e] = m[rt][e] == mn ? 1.f : (m[rt][e] == -INFINITY ? 0.f : exp2_fast(m[rt][e] - mn));
+            const float d = m[rt][e] == mn ? 0.f : m[rt][e] - mn;
+            corr[e] = exp2_fast(d);
             m[rt][e] = mn;
-            l[rt][e] *= corr[e];
+            l[rt][e] = scale_sum(l[rt][e], d);
           }
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt)
@@ -465,6 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
             for (int e = 0; e < 4; ++e) o[rt][mt][e] *= corr[e & 1];
         }
       }
+      const bool tiny = vs_now < kTinyScale;
       uint32_t pf[RT][2][2];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
@@ -472,6 +474,12 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
         for (int e = 0; e < 2; ++e) {
           const float ref = m[rt][e] == -INFINITY ? 0.f : m[rt][e] - 10.f;
           float add = 0.f;
+          if (tiny) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int hh = 0; hh < 4; hh += 2) l[rt][e] = fmaf(exp2_fast(s[rt][mt][e + hh] - (ref + ev)), kSumUnit, l[rt][e]);
+          }
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -480,7 +488,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
               s[rt][mt][e + hh] = x;
               add += x;
             }
-          l[rt][e] = fmaf(add, vi, l[rt][e]);
+          if (!tiny) l[rt][e] = fmaf(add, vi, l[rt][e]);
         }
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
@@ -551,14 +559,14 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) {
         const float mw = red[x][r][D];
-        const float f = mw == -INFINITY && M != -INFINITY ? 0.f : (M == -INFINITY ? 1.f : exp2_fast(mw - M));
-        L += red[x][r][D + 1] * f;
+        const float d = M == -INFINITY ? 0.f : mw - M, f = exp2_fast(d);
+        L += scale_sum(red[x][r][D + 1], d);
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] += red[x][r][c + e] * f;
       }
       if (whole) {
         const int rr = row0 + r, i = rr / p.group;
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float inv = L == 0.f ? 0.f : kSumUnit / L;
         const uint2 y = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
         __nv_bfloat16* dst =
             p.out + b * p.o_sb + (static_cast<long long>(i) * p.H + hk * p.group + rr - i * p.group) * D + c;
@@ -614,8 +622,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cache_attn_merge_kernel(cons
 #pragma unroll 8
     for (int c = first; c <= cut.more; c += by) {
       const float* x = slot(c);
-      const float f = M == -INFINITY ? 1.f : exp2_fast(x[D] - M);
-      L += x[D + 1] * f;
+      const float d = M == -INFINITY ? 0.f : x[D] - M, f = exp2_fast(d);
+      L += scale_sum(x[D + 1], d);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
         const float2 y = *reinterpret_cast<const float2*>(x + lane * N + e);
@@ -624,7 +632,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cache_attn_merge_kernel(cons
       }
     }
     if (few) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float inv = L == 0.f ? 0.f : kSumUnit / L;
 #pragma unroll
       for (int e = 0; e < N; e += 2) store_row<D>(p, cut, r, lane * N + e, a[e] * inv, a[e + 1] * inv);
       continue;
@@ -642,12 +650,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cache_attn_merge_kernel(cons
       for (int w = 0; w < kMergeWarps; ++w) mx = fmaxf(mx, red[w][D]);
 #pragma unroll
       for (int w = 0; w < kMergeWarps; ++w) {
-        const float f = mx == -INFINITY ? 1.f : exp2_fast(red[w][D] - mx);
-        l += red[w][D + 1] * f;
+        const float d = mx == -INFINITY ? 0.f : red[w][D] - mx, f = exp2_fast(d);
+        l += scale_sum(red[w][D + 1], d);
         x0 = fmaf(red[w][2 * threadIdx.x], f, x0);
         x1 = fmaf(red[w][2 * threadIdx.x + 1], f, x1);
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : kSumUnit / l;
       store_row<D>(p, cut, r, 2 * threadIdx.x, x0 * inv, x1 * inv);
     }
     __syncthreads();

@@ -16,6 +16,22 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Row sums. A key's weight is w = 2^(s + ev - m + c), m the running maximum of s + ev (lagging by up to 8) and c a
+// constant; the row sum adds w 2^-ev. V's scales 2^ev lie in [2^-100, 2^120], so a key's part of the sum lies between
+// 2^(c - 120) for the maximum itself and 2^(c + 8 + 100). Counted in units of 2^13 neither end leaves fp32's normal
+// range, for up to 2^25 keys.
+constexpr float kSumUnit = 0x1p-13f;
+// A block of tiny values (of zeros above all: 2^-100) beside large ones: w itself leaves fp32's range before its part
+// of the sum is negligible, so blocks under this scale add exp2(s - m + c) on its own. What is left out then needs
+// two blocks of one row whose scales are 2^115 and more apart, the smaller one above this.
+constexpr float kTinyScale = 0x1p-60f;
+
+// sum * 2^d for d <= 0: the sum may be as large as 2^-d, so that 2^d alone would be zero too early.
+__device__ __forceinline__ float scale_sum(float sum, float d) {
+  const float h = exp2_fast(0.5f * d);
+  return sum * h * h;
+}
+
 // Two e4m3 bytes -> two halves (exact).
 __device__ __forceinline__ uint32_t f16x2_of(uint32_t two_bytes) {
   uint32_t d;

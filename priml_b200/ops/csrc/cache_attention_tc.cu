@@ -54,6 +54,7 @@ constexpr int kLaunch = 640;  // whole warpgroups, so that the register split be
 // Registers per thread after the split; 640 threads are launched with 96 each.
 constexpr int kRegsSoftmax = 136, kRegsConvert = 72, kRegsIssue = 64;
 static_assert(256 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsIssue <= kLaunch * 96, "register split");
+constexpr float kTinyLog2 = -60.f;  // log2 of kTinyScale
 constexpr float kShift = 7.f;     // weights are up to 2^(threshold + shift) = 2^15, within f16
 // An item's start and end cost a CTA about as much as this many key tiles. Without it CTAs with many short items
 // ran long: five tokens each of 8 ragged sequences 116 us (with it 72), four windowed prompts of 1111 tokens, 576
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ long long warp_sum[kLaunch / 32];
   __shared__ uint32_t v_bad[NS][kConvertWarps][4];  // keys of an edge tile whose values hold a NaN
-  __shared__ alignas(16) float scales[NS][12];      // per 32 keys: K's scale, log2 of V's, its reciprocal
+  __shared__ alignas(16) float scales[NS][12];      // per 32 keys: K's scale, log2 of V's, kSumUnit over V's
   __shared__ Piece pieces[kPieces];
   __shared__ Walk walk;
 
@@ -461,7 +462,8 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         const float2 ve2 = *reinterpret_cast<const float2*>(&scales[st][4 + 2 * half]);
         const float2 vi2 = *reinterpret_cast<const float2*>(&scales[st][8 + 2 * half]);
         const float kc[2] = {fmaxf(factor * ks2.x, 1e-37f), fmaxf(factor * ks2.y, 1e-37f)};
-        const float ve[2] = {ve2.x, ve2.y}, vi[2] = {vi2.x, vi2.y};
+        const float ve[2] = {ve2.x, ve2.y};
+        float vi[2] = {vi2.x, vi2.y};
         uint32_t va[32], vb[32];
         tmem_read_x32x2(tB, va, vb);
         if (k0 > edge_hi || k0 < edge_lo) {
@@ -499,8 +501,8 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           // the last step's product must be in O; the one after it waits for this step's weights
           if (!(ok = mbar_wait_warp(&pv_done[t], (n_pv - 1) & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
           tc_fence_after();
-          const float f = scale_o ? fast_exp2(m - mx) : 1.f;
-          l *= f;
+          const float d = scale_o ? m - mx : 0.f, f = fast_exp2(d);
+          l = scale_sum(l, d);
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
@@ -512,6 +514,17 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         }
         if (grow) m = mx;
         const float ref = m == -INFINITY ? 0.f : kShift - m;
+        // (one branch ahead of both halves: within them it cost 3 % of a long chunk's time)
+        if (__builtin_expect(fminf(ve[0], ve[1]) < kTinyLog2, 0)) {
+          auto sum_alone = [&](const uint32_t(&v)[32], int c) {
+            if (!(ve[c] < kTinyLog2)) return;
+            vi[c] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) l = fmaf(fast_exp2(fmaf(__uint_as_float(v[i]), kc[c], ref)), kSumUnit, l);
+          };
+          sum_alone(va, 0);
+          sum_alone(vb, 1);
+        }
         auto weigh = [&](const uint32_t(&v)[32], int c) {
           const float add = ref + ve[c];
           const uint64_t mul2 = f2_pack(kc[c], kc[c]), add2 = f2_pack(add, add);
@@ -558,14 +571,15 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         if (t == 0) {
           const float m2 = scratch[0], l2 = scratch[1];
           const float mm = fmaxf(m, m2);
-          f_own = m == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : fast_exp2(m - mm);
-          f_other = m2 == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : fast_exp2(m2 - mm);
-          l = l * f_own + l2 * f_other;
+          const float d = mm == -INFINITY ? 0.f : m - mm, d2 = mm == -INFINITY ? 0.f : m2 - mm;
+          f_own = fast_exp2(d);
+          f_other = fast_exp2(d2);
+          l = scale_sum(l, d) + scale_sum(l2, d2);
           m = mm;
         }
         meet();
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : kSumUnit / l;
       float* part = p.part + ((2LL * blockIdx.x + x.begins) * kCacheTcRows + (both ? r : t * 128 + r)) * (D + 2);
       __nv_bfloat16* orow = p.out + x.b * p.o_sb + (static_cast<long long>(write ? tok : 0) * p.H + (write ? head : 0)) * D;
       if (write && !whole) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
@@ -669,7 +683,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         if (!(ok = mbar_wait_warp(&empty[st], ((tile_no / NS) & 1) ^ 1u, p.status, kTimeoutProducer, abort_flag))) break;
         if (brings) {
           scales[st][c] = c < 4 ? sc : __log2f(sc);
-          if (c >= 4) scales[st][4 + c] = 1.f / sc;
+          if (c >= 4) scales[st][4 + c] = kSumUnit / sc;
           if (j + 1 < count) sc = scale_at(k0 + kKeys);
         }
         if (is_v && (k0 > edge_hi || k0 < edge_lo)) {

@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch import Tensor
 
-from tests.cache8_cases import filled_cache
+from tests.cache8_cases import BLOCK, attend64, filled_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -25,6 +25,16 @@ def _queries(b: int, s: int, h: int, d: int, seed: int) -> Tensor:
 
 def _ints(values: list[int]) -> Tensor:
     return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _limit(want: Tensor, spread: Tensor) -> Tensor:
+    """How far a kernel's output may be from 64 bits: ``spread`` is the same attention over |V|.
+
+    Each weight p is rounded to f16, half a step being 2**-11 of it, and the sum of p is not rounded with it: 2**-11 of
+    sum p |V|. Scores of up to 2**7 are off by a few 2**-24 of their size, weights by less than 2**-15, numerator and
+    sum alike: 2**-14 more. The rounding to bf16 is half a step of an 8-bit significand: 2**-8 of the result.
+    """
+    return want.abs() * 2.0**-8 + spread * (2.0**-11 + 2.0**-13) * (1 + 2.0**-8)
 
 
 @pytest.mark.parametrize("shift", [0, 14, 20, 100])
@@ -45,3 +55,28 @@ def test_queries_before_their_sequence_give_zeros_whatever_the_scales(b, s, h, h
     # the shift moves exponents by roundings only: neighbours in bf16, 2**-7 apart, but where terms cancel
     size = (v.float().abs().amax((-1, -2)) * vs.amax(-1)).max()
     assert ((out.float() * 2.0**-shift - base.float()).abs() <= base.float().abs() * 2.0**-7 + size * 2.0**-16).all()
+
+
+@pytest.mark.parametrize("s", [1, 5, 150])
+@pytest.mark.parametrize("large", [7, 20, 40, 90])
+@pytest.mark.parametrize("zero_first", [True, False])
+def test_blocks_of_zeros_beside_large_values(s: int, large: int, zero_first: bool) -> None:
+    """A block of zeros has the least scale, 2**-100; its keys count in the sum of the weights all the same."""
+    from priml_b200 import ops
+
+    b, h, hkv, t, d = 2, 8, 2, 700, 64
+    k, ks = filled_cache(b, hkv, t, d, seed=11, device="cuda")
+    v, vs = filled_cache(b, hkv, t, d, seed=12, device="cuda")
+    q = _queries(b, s, h, d, seed=13)
+    zero = (torch.arange(-(-t // BLOCK), device="cuda") % 3 == 1) ^ (torch.arange(-(-t // BLOCK), device="cuda") < 6)
+    if not zero_first:
+        zero = ~zero
+    rows = zero.repeat_interleave(BLOCK)[:t]
+    v.view(torch.uint8)[:, :, rows] = 0
+    vs[:, :, zero], vs[:, :, ~zero] = 2.0**-100, vs[:, :, ~zero] * 2.0**large
+    ends = [t, 400]
+    out = ops.cache_attention(q, k, v, ks, vs, _ints(ends)).cpu().double()
+    _status_clean()
+    want = attend64(q, k, v, ks, vs, ends)
+    spread = attend64(q, k, v.float().abs().to(v.dtype), ks, vs, ends)
+    assert ((out - want).abs() <= _limit(want, spread)).all()
