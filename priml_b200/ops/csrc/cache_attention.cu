@@ -386,27 +386,37 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
       }
       const bool edge = base_row + kCacheBlock - 1 > lo_max || base_row < hi_min;
       if (edge) {
-        // A value row may hold NaN where only some rows see it: its bytes become zero, and the
-        // scores of the rows that do see it become NaN.
-        uint32_t bad = 0;  // bit i: key i of vr has a NaN in this lane's channels
+        // A value row may hold NaN where only some rows see it: its bytes become zero, and the channel becomes
+        // NaN in the rows that do see it (elsewhere the products see to that).
+        uint32_t bad[8];  // bit c: channel g * D / 8 + c of key i of vr
+        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint32_t any = 0;
+          bad[i] = 0;
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) {
-            const uint32_t nb8 = nan_bytes(vr[i][w]);
-            vr[i][w] &= ~nb8;
-            any |= nb8;
-          }
-          bad |= any != 0 ? 1u << i : 0u;
+          for (int w = 0; w < D / 32; ++w) bad[i] |= nan_bits(vr[i][w]) << (4 * w);
+          any |= bad[i];
         }
-        uint32_t badrows = 0;  // bit per key of the step, over the whole warp
-        if (__any_sync(0xffffffffu, bad != 0)) {
-          uint32_t mine = 0;
+        if (__any_sync(0xffffffffu, any != 0)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (bad >> i & 1) mine |= 1u << ((i >> 2) * 16 + ((i >> 1) & 1) * 8 + key_of<D>(2 * t + (i & 1)));
-          badrows = __reduce_or_sync(0xffffffffu, mine);
+          for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) vr[i][w] &= ~nan_bytes(vr[i][w]);
+#pragma unroll 1
+            for (int src = 0; src < 4; ++src) {  // the lane of this quad's channels that holds the key's bytes
+              const uint32_t m = __shfl_sync(0xffffffffu, bad[i], (lane & ~3) | src);
+              const int key = base_row + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + key_of<D>(2 * src + (i & 1));
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (m != 0 && key <= kmax[rt][e] && key >= kmin[rt][e]) {
+#pragma unroll
+                    for (int c = 0; c < D / 8; ++c)
+                      if (m >> c & 1) o[rt][c >> 1][e + 2 * (c & 1)] = NAN;
+                  }
+            }
+          }
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -414,9 +424,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int in = mt * 16 + (e >> 1) * 8 + key_of<D>(g);
-              const int key = base_row + in;
-              if (badrows >> in & 1) s[rt][mt][e] = NAN;
+              const int key = base_row + mt * 16 + (e >> 1) * 8 + key_of<D>(g);
               if (key > kmax[rt][e & 1] || key < kmin[rt][e & 1]) s[rt][mt][e] = -INFINITY;
             }
       }

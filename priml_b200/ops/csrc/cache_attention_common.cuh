@@ -66,6 +66,11 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return (m >> 7) * 255u;
 }
 
+// Bit i: byte i of `w` is an e4m3 NaN.
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) {
+  return ((nan_bytes(w) & 0x01010101u) * 0x01020408u) >> 24 & 15u;
+}
+
 // A query row whose largest magnitude is `amax` fits f16 after the exact factor `down`; `up` undoes it.
 // Rows that are zero, tiny or not finite stay as they are.
 __device__ __forceinline__ void row_power(float amax, float& down, float& up) {

@@ -201,6 +201,7 @@ struct Piece {
   int from[2], to[2];    // tiles of the piece that row tile 0 / 1 sees
   int both;              // at most 128 rows: the groups share them and take half of each tile
   int whole, begins;     // the piece is the whole item; it holds the item's first tile
+  int nan;               // an edge tile of the piece holds a value that is NaN (set by V's converting warps)
 };
 
 // Walks a CTA's run of the list (one thread; its state lies in shared memory, not in registers).
@@ -256,6 +257,7 @@ struct Walk {
     x.both = p.s * p.group - x.row0 <= 128;
     x.whole = j0 == 0 && j1 == sp.count;
     x.begins = j0 == 0;
+    x.nan = 0;
     for (int t = 0; t < 2; ++t) {
       const Span st = span_of(p, b, x.row0 + 128 * t, 128);
       x.from[t] = max(st.first - x.kt0, 0);
@@ -264,6 +266,29 @@ struct Walk {
     if (j0 == 0 && j1 < sp.count) cut = {b, hk, x.row0, static_cast<int>((sp.count - j1 + run - 1) / run)};
   }
 };
+
+// NaNs in the values of a piece's edge tiles are zero in shared memory. This makes their channels NaN in the stored result
+// of a row at position `pos` that sees them, reading the cache again (and the piece from shared memory: nothing here
+// may live in registers while the softmax runs).
+template <int D>
+__device__ __forceinline__ void store_nans(const CacheAttnParams& p, const Piece& x, int pos, __nv_bfloat16* out, float* part) {
+  const uint8_t* rows = p.v + x.b * p.v_sb + x.hk * p.v_sh;
+  const int kmin = p.window >= 0 ? pos - p.window : 0;
+#pragma unroll 1
+  for (int k0 = x.kt0 * kKeys; k0 < (x.kt0 + x.count) * kKeys; k0 += kKeys) {
+    if (k0 <= x.edge_hi && k0 >= x.edge_lo) continue;
+#pragma unroll 1
+    for (int key = max(k0, kmin); key <= min(k0 + kKeys - 1, pos); ++key) {
+      const uint8_t* row = rows + static_cast<long long>(key) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; ++c) {
+        if ((row[c] & 0x7f) != 0x7f) continue;
+        if (x.whole) out[c] = __float2bfloat16_rn(NAN);
+        else part[c] = NAN;
+      }
+    }
+  }
+}
 
 template <int D>
 __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAttnParams p) {
@@ -292,7 +317,6 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ long long warp_sum[kLaunch / 32];
-  __shared__ uint32_t v_bad[NS][kConvertWarps][4];  // keys of an edge tile whose values hold a NaN
   __shared__ alignas(16) float scales[NS][12];      // per 32 keys: K's scale, log2 of V's, kSumUnit over V's
   __shared__ Piece pieces[kPieces];
   __shared__ Walk walk;
@@ -454,7 +478,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         if (!(ok = mbar_wait_warp(&s_full[2 * t + buf], s_phase >> buf & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
         s_phase ^= 1u << buf;
         tc_fence_after();
-        // the tile's scales (and the flags below) come with its values
+        // the tile's scales come with its values
         const uint32_t tile_no = tiles_before + j;
         const int st = tile_no % NS;
         if (!(ok = mbar_wait_warp(&v_full[st], (tile_no / NS) & 1, p.status, kTimeoutEpilogue, abort_flag))) break;
@@ -468,17 +492,9 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         tmem_read_x32x2(tB, va, vb);
         if (k0 > edge_hi || k0 < edge_lo) {
           auto mask = [&](uint32_t(&v)[32], int c) {  // scores of keys 32c .. 32c + 31 of the tile
-            uint32_t bad = 0;
-#pragma unroll
-            for (int w = 0; w < kConvertWarps; ++w) bad |= v_bad[st][w][c];
             // bit i: the row sees key i of these
             const int hi = kmax - k0 - 32 * c, lo = kmin - k0 - 32 * c;
             const uint32_t sees = (hi < 0 ? 0u : hi > 30 ? ~0u : (2u << hi) - 1u) & (lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo);
-            if (bad != 0) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (bad >> i & 1) v[i] = 0x7fffffffu;
-            }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!(sees >> i & 1)) v[i] = __float_as_uint(-INFINITY);
@@ -627,6 +643,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           for (int i = 0; i < 16; ++i) *reinterpret_cast<float2*>(part + c * 32 + 2 * i) = make_float2(y[2 * i], y[2 * i + 1]);
         }
       }
+      if (write && x.nan) store_nans<D>(p, x, x.base + tok, orow, part);
       if (!ok) break;
       tiles_before += count;
       tc_fence_before();
@@ -652,7 +669,7 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
     bool ok = true;
     for (uint32_t seg = 0; ok; ++seg) {
       if (!(ok = mbar_wait_warp(&piece_full[seg % kPieces], (seg / kPieces) & 1, p.status, kTimeoutProducer, abort_flag))) break;
-      const Piece& x = pieces[seg % kPieces];
+      Piece& x = pieces[seg % kPieces];
       const int count = x.count;
       if (count == 0) break;
       const int n_keys = x.n, edge_hi = x.edge_hi, edge_lo = x.edge_lo;
@@ -687,20 +704,15 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
           if (j + 1 < count) sc = scale_at(k0 + kKeys);
         }
         if (is_v && (k0 > edge_hi || k0 < edge_lo)) {
-          // an edge tile: values that are NaN become zero, their keys are told to the softmax
-          uint32_t bad[4] = {0, 0, 0, 0};
+          // an edge tile: values that are NaN become zero here, and the rows' ends are told to look for them
+          uint32_t any = 0;
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
             const uint32_t a = nan_bytes(raw[i].x), b2 = nan_bytes(raw[i].y), c2 = nan_bytes(raw[i].z), d2 = nan_bytes(raw[i].w);
             raw[i] = make_uint4(raw[i].x & ~a, raw[i].y & ~b2, raw[i].z & ~c2, raw[i].w & ~d2);
-            const int row = row_c + i * (128 / PR);
-            if (a | b2 | c2 | d2) bad[(i * (128 / PR)) >> 5] |= 1u << (row & 31);
+            any |= a | b2 | c2 | d2;
           }
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t all = __reduce_or_sync(0xffffffffu, bad[w]);
-            if (lane == 0) v_bad[st][warp - kSoftmaxWarps - kConvertWarps][w] = all;
-          }
+          if (any != 0) x.nan = 1;
         }
         uint8_t* tile = tiles + st * C::kQTile;
 #pragma unroll

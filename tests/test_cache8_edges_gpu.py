@@ -80,3 +80,37 @@ def test_blocks_of_zeros_beside_large_values(s: int, large: int, zero_first: boo
     want = attend64(q, k, v, ks, vs, ends)
     spread = attend64(q, k, v.float().abs().to(v.dtype), ks, vs, ends)
     assert ((out - want).abs() <= _limit(want, spread)).all()
+
+
+@pytest.mark.parametrize("b,s,h,hkv,t,d,ends,window", [
+    (2, 1, 8, 2, 300, 128, [300, 270], None),
+    (2, 1, 16, 1, 300, 64, [300, 17], 60),
+    (2, 5, 4, 2, 300, 64, [300, 270], None),
+    (2, 5, 8, 1, 300, 128, [290, 31], 40),  # a group of 8: the many-row form, both groups on the same rows
+    (2, 150, 4, 2, 300, 64, [300, 270], None),
+    (2, 150, 4, 2, 300, 128, [300, 100], 60),
+    (1, 700, 2, 1, 4500, 128, [4444], None),  # runs that are cut and joined
+])  # fmt: skip
+def test_a_value_that_is_nan_stays_in_its_channel(b, s, h, hkv, t, d, ends, window) -> None:  # noqa: ANN001
+    from priml_b200 import ops
+    from priml_b200.ops import reference
+
+    k, ks = filled_cache(b, hkv, t, d, seed=31, device="cuda")
+    v, vs = filled_cache(b, hkv, t, d, seed=32, device="cuda")
+    q = _queries(b, s, h, d, seed=33)
+    g = torch.Generator().manual_seed(34)
+    bits = v.view(torch.uint8)
+    at = [(i, int(torch.randint(hkv, (), generator=g)), max(0, ends[i] - 1 - back), int(torch.randint(d, (), generator=g)))
+          for i in range(b) for back in (0, 1, 7, s - 1, s + 20, 90)]  # fmt: skip
+    for where in at:
+        bits[where] = 0
+    clean = ops.cache_attention(q, k, v, ks, vs, _ints(ends), window=window)
+    for n, where in enumerate(at):
+        bits[where] = 0x7F if n % 2 else 0xFF
+    out = ops.cache_attention(q, k, v, ks, vs, _ints(ends), window=window)
+    _status_clean()
+    want = reference.cache_attention(
+        *(x.cpu() for x in (q.float(), k, v, ks, vs, _ints(ends))), scale=d**-0.5, window=window
+    ).isnan()
+    assert torch.equal(out.cpu().isnan(), want) and want.any() and not want.all()
+    assert torch.equal(out[~want.cuda()], clean[~want.cuda()])
