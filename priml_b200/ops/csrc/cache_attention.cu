@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(kWarps * 32, (Cfg<D, RT>::kCtas)) cache_attn_k
               s[rt][mt][e + hh] = x;
               add += x;
             }
-          if (!tiny) l[rt][e] = fmaf(add, vi, l[rt][e]);
+          // (a row that sees nothing of the step adds nothing, whatever the block's scale holds)
+          if (!tiny && add != 0.f) l[rt][e] = fmaf(add, vi, l[rt][e]);
         }
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {

@@ -156,6 +156,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
       : "memory");
 }
 
+// x, at least 1e-37 (a hidden key's -inf must stay -inf times this); NaN stays NaN.
+__device__ __forceinline__ float positive(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(1e-37f));
+  return x;
+}
+
 __device__ __forceinline__ bool elect_one() {
   uint32_t e;
   asm volatile(
@@ -485,8 +491,8 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
         const float2 ks2 = *reinterpret_cast<const float2*>(&scales[st][2 * half]);
         const float2 ve2 = *reinterpret_cast<const float2*>(&scales[st][4 + 2 * half]);
         const float2 vi2 = *reinterpret_cast<const float2*>(&scales[st][8 + 2 * half]);
-        const float kc[2] = {fmaxf(factor * ks2.x, 1e-37f), fmaxf(factor * ks2.y, 1e-37f)};
-        const float ve[2] = {ve2.x, ve2.y};
+        float kc[2] = {positive(factor * ks2.x), positive(factor * ks2.y)};
+        float ve[2] = {ve2.x, ve2.y};
         float vi[2] = {vi2.x, vi2.y};
         uint32_t va[32], vb[32];
         tmem_read_x32x2(tB, va, vb);
@@ -498,6 +504,10 @@ __global__ void __launch_bounds__(kLaunch, 1) cache_attn_tc_kernel(const CacheAt
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!(sees >> i & 1)) v[i] = __float_as_uint(-INFINITY);
+            if (sees == 0) {  // the row's weights are zero whatever the block's scales hold
+              kc[c & 1] = 1.f;
+              ve[c & 1] = vi[c & 1] = 0.f;
+            }
           };
           mask(va, 2 * half);
           mask(vb, 2 * half + 1);

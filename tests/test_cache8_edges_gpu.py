@@ -114,3 +114,26 @@ def test_a_value_that_is_nan_stays_in_its_channel(b, s, h, hkv, t, d, ends, wind
     ).isnan()
     assert torch.equal(out.cpu().isnan(), want) and want.any() and not want.all()
     assert torch.equal(out[~want.cuda()], clean[~want.cuda()])
+
+
+@pytest.mark.parametrize("s", [1, 6, 150])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_scale_that_is_nan_reaches_the_queries_that_see_its_block(s: int, which: str) -> None:
+    from priml_b200 import ops
+    from priml_b200.ops import reference
+
+    b, h, hkv, t, d = 2, 8, 2, 330, 64
+    k, ks = filled_cache(b, hkv, t, d, seed=21, device="cuda")
+    v, vs = filled_cache(b, hkv, t, d, seed=22, device="cuda")
+    q, ends = _queries(b, s, h, d, seed=23), [330, 200]
+    clean = ops.cache_attention(q, k, v, ks, vs, _ints(ends), window=40)
+    scale = ks if which == "k" else vs
+    scale[0, 1, (330 - s // 2) // BLOCK] = float("nan")
+    scale[1, 0, 170 // BLOCK] = float("nan")
+    out = ops.cache_attention(q, k, v, ks, vs, _ints(ends), window=40)
+    _status_clean()
+    want = reference.cache_attention(
+        *(x.cpu() for x in (q.float(), k, v, ks, vs, _ints(ends))), scale=d**-0.5, window=40
+    ).isnan()
+    assert torch.equal(out.cpu().isnan(), want) and want.any() and not want.all()
+    assert torch.equal(out[~want.cuda()], clean[~want.cuda()])
