@@ -34,8 +34,8 @@
 //                  B: P^T from S^T by an 8 x 8 transpose (movmatrix).
 // One scale belongs to one 32-key step: K's multiplies the scores; V's goes into the weights,
 // w = 2^(s + ev - m), m the running maximum of s + ev, while the row sum adds w 2^-ev. So the weights
-// fit f16 whatever the scales. Query rows are normalised by a power of two to fit f16 (exact; the
-// factor goes to the scores). Weights are rounded to f16 as 2^10 w: half a step is 2^-11 relative down
+// fit f16 whatever the scales. Query rows are normalised by a power of two to fit f16 (exact down to 2^-30
+// of the row's largest channel, see row_power; the factor goes to the scores). Weights are rounded to f16 as 2^10 w: half a step is 2^-11 relative down
 // to w = 2^-24, less than bf16's 2^-9 of the output, and far tails stay above zero.
 //
 // Work split: the key blocks of all (sequence, KV head, row group) items form one list, cut into

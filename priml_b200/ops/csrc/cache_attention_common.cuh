@@ -71,13 +71,16 @@ __device__ __forceinline__ uint32_t nan_bits(uint32_t w) {
   return ((nan_bytes(w) & 0x01010101u) * 0x01020408u) >> 24 & 15u;
 }
 
-// A query row whose largest magnitude is `amax` fits f16 after the exact factor `down`; `up` undoes it.
-// Rows that are zero, tiny or not finite stay as they are.
+// A query row times the power of two `down` fits f16; `up` undoes it. The row's largest magnitude goes to [2^13, 2^14):
+// f16 ends at 2^16 and its least step is 2^-24, so channels down to 2^-30 of the largest keep all their bits (bf16 has
+// eight) and smaller ones are off by at most 2^-38 of the largest. Zero rows and rows with an infinity stay as they are;
+// rows under 2^-113 go as far up as `up` stays a normal number.
 __device__ __forceinline__ void row_power(float amax, float& down, float& up) {
   const uint32_t ex = (__float_as_uint(amax) >> 23) & 255u;
-  const bool plain = ex < 2u || ex > 252u;
-  down = plain ? 1.f : __uint_as_float((254u - ex) << 23);
-  up = plain ? 1.f : __uint_as_float(ex << 23);
+  const bool plain = ex == 0u || ex == 255u;
+  const uint32_t lift = min(13u, ex - 1u);
+  down = plain ? 1.f : __uint_as_float((254u - ex + lift) << 23);
+  up = plain ? 1.f : __uint_as_float((ex - lift) << 23);
 }
 
 // Keys of sequence b in the launch's view (what follows its last token taken off); may be negative.

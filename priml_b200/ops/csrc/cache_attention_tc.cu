@@ -13,7 +13,7 @@
 // The block scales never touch the tiles: K's multiplies the scores of its 32 keys as part of the
 // exponent's multiply-add; V's goes into the weights, w = 2^(s + ev - M), M being the running maximum
 // of s + ev, so that w is within f16 whatever the scales, and the row sum adds w 2^-ev. Queries are
-// normalised by a power of two per row to fit f16.
+// normalised by a power of two per row to fit f16 (exact down to 2^-30 of the row's largest channel).
 //
 //   warps 0-3, 4-7   softmax of row tiles 0 and 1 (one row per thread); they also load their Q rows
 //   warps 8-11       K tiles, e4m3 -> f16: 16-byte loads a tile ahead, held in registers

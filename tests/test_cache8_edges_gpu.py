@@ -137,3 +137,47 @@ def test_a_scale_that_is_nan_reaches_the_queries_that_see_its_block(s: int, whic
     ).isnan()
     assert torch.equal(out.cpu().isnan(), want) and want.any() and not want.all()
     assert torch.equal(out[~want.cuda()], clean[~want.cuda()])
+
+
+@pytest.mark.parametrize("s", [1, 6, 150])
+@pytest.mark.parametrize("power", [0, 16, 22])
+def test_an_outlying_query_channel_leaves_the_others_their_bits(s: int, power: int) -> None:
+    """One channel of the queries is 2**power times the others and meets keys that are zero there."""
+    from priml_b200 import ops
+
+    b, h, hkv, t, d = 1, 4, 2, 300, 64
+    k, ks = filled_cache(b, hkv, t, d, seed=41, device="cuda")
+    v, vs = filled_cache(b, hkv, t, d, seed=42, device="cuda")
+    k.view(torch.uint8)[..., 5] = 0
+    q = _queries(b, s, h, d, seed=43) * 8  # scores of some tens: a relative 2**-8 of one would show
+    plain = q.clone()
+    q[..., 5] = 2.0**power
+    plain[..., 5] = 0
+    out = ops.cache_attention(q, k, v, ks, vs, _ints([t])).cpu().double()
+    _status_clean()
+    want = attend64(plain, k, v, ks, vs, [t])
+    spread = attend64(plain, k, v.float().abs().to(v.dtype), ks, vs, [t])
+    assert ((out - want).abs() <= _limit(want, spread)).all()
+
+
+@pytest.mark.parametrize("s", [1, 6, 150])
+@pytest.mark.parametrize("size", [-100, 60, 127])
+def test_queries_of_any_finite_size(s: int, size: int) -> None:
+    from priml_b200 import ops
+
+    b, h, hkv, t, d = 1, 4, 2, 300, 64
+    k, ks = filled_cache(b, hkv, t, d, seed=44, device="cuda")
+    v, vs = filled_cache(b, hkv, t, d, seed=45, device="cuda")
+    q = _queries(b, s, h, d, seed=46)
+    base = ops.cache_attention(q, k, v, ks, vs, _ints([t]))
+    far = (q.float() * 2.0**size).bfloat16()
+    assert far.isfinite().all()
+    out = ops.cache_attention(far, k, v, ks, vs, _ints([t]), scale=d**-0.5 * 2.0**-size)
+    _status_clean()
+    if size < 120:  # powers of two all along: the same bits
+        assert torch.equal(out, base)
+        return
+    # scale * log2(e) is 2**-129.5, a subnormal fp32 number: half a step, 2**-150, is 2**-20 of it. Scores stay under 2**6,
+    # so exponents are off by 2**-14, numerator and sum by 2**-14 of themselves; the roundings to bf16 may then be neighbours.
+    size_v = (v.float().abs().amax((-1, -2)) * vs.amax(-1)).max()
+    assert ((out.float() - base.float()).abs() <= base.float().abs() * 2.0**-7 + 2.0**-13 * size_v).all()
