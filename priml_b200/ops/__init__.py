@@ -106,7 +106,7 @@ def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, interleave: bool =
     have a head axis of their own; the first ``R`` channels of a head are rotated, the others copied.
     The pairs are channels ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleave``. The rotation is
     computed in fp32 and rounded once. On CUDA q and k take one kernel (bf16, fp16, fp32), and its
-    transpose in the backward; factors that need a gradient take the torch operations.
+    transpose in the backward; odd head widths and factors that need a gradient take the torch operations.
     """
     if use_native(q):
         from priml_b200.ops import functional

@@ -724,6 +724,7 @@ std::vector<Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& cos, 
   const auto st = q.scalar_type();
   PB_CHECK(st == torch::kBFloat16 || st == torch::kFloat32 || st == torch::kFloat16, "q must be bf16, fp16 or fp32");
   const int64_t B = q.size(0), S = q.size(1), H = q.size(2), Hk = k.size(2), D = q.size(3);
+  PB_VALUE(D % 2 == 0, "the head dim must be even");  // units of two vectors: an odd channel would not be written
   PB_CHECK(q.stride(3) == 1 && k.stride(3) == 1, "channels must be contiguous");
   PB_CHECK(cos.sizes() == sin.sizes() && (cos.dim() == 3 || cos.dim() == 4), "cos and sin must be [(B,) S, heads, R/2]");
   auto c = aux(cos, q, torch::kFloat32);

@@ -161,7 +161,7 @@ void launch_rotary_v(const RotaryParams& all, cudaStream_t stream) {
   }
 }
 
-// Widest vector that the channel counts, strides and base addresses all allow.
+// Widest vector that the channel counts, strides and base addresses all allow. (D is even.)
 template <typename T>
 void launch_rotary(const RotaryParams& p, cudaStream_t stream) {
   auto fits = [&](int v) {

@@ -418,6 +418,7 @@ def rotary_any_supported(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> bool
         and q.dtype in (torch.bfloat16, torch.float16, torch.float32)
         and q.shape[:2] == k.shape[:2]
         and q.shape[-1] == k.shape[-1]
+        and q.shape[-1] % 2 == 0  # the kernel moves channels by twos
         and q.shape[0] * q.shape[1] < 1 << 31
         and (q.shape[2] + k.shape[2]) * q.shape[3] < 1 << 22
         and cos.shape == sin.shape
