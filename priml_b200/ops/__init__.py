@@ -106,14 +106,15 @@ def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, interleave: bool =
     have a head axis of their own; the first ``R`` channels of a head are rotated, the others copied.
     The pairs are channels ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleave``. The rotation is
     computed in fp32 and rounded once. On CUDA q and k take one kernel (bf16, fp16, fp32), and its
-    transpose in the backward; odd head widths and factors that need a gradient take the torch operations.
+    transpose in the backward; odd head widths and factors that need a gradient take the torch operations,
+    and so do calls under ``torch.func`` transforms, forward-mode AD, ``torch.compile`` and fake tensors.
     """
     if use_native(q):
         from priml_b200.ops import functional
 
         if not interleave and q.dtype == torch.bfloat16 and cos.ndim == 3 and cos.shape[-1] * 2 == q.shape[-1] and cos.shape[-2] == 1:
             return functional.rotary(q, k, cos, sin)
-        if functional.rotary_any_supported(q, k, cos, sin):
+        if functional.rotary_any_supported(q, k, cos, sin) and not functional.traced(q, k, cos, sin):
             return native().rotary(q, k, cos, sin, interleave)
     return reference.rotate(q, cos, sin, interleave), reference.rotate(k, cos, sin, interleave)
 

@@ -15,6 +15,7 @@ import math
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from priml_b200.ops._loader import native
 
@@ -405,6 +406,16 @@ class _Rotary(torch.autograd.Function):
         c, s = ctx.saved_tensors
         n = native()
         return n.rope(dq.contiguous(), c, s, -1.0), n.rope(dk.contiguous(), c, s, -1.0), None, None
+
+
+def traced(*tensors: Tensor) -> bool:
+    """Whether a compiled autograd node must not see these tensors: something else than their data is wanted of them."""
+    return (
+        torch.compiler.is_compiling()
+        or torch._C._are_functorch_transforms_active()
+        or any(type(t) not in (Tensor, torch.nn.Parameter) for t in tensors)
+        or (forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+    )
 
 
 def rotary_any_supported(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> bool:
