@@ -133,26 +133,43 @@ def cache_append(x: Tensor, cache: Tensor, scale: Tensor, lengths: Tensor) -> No
 
     A block of 32 rows that held rows before keeps its scale unless the new rows need a larger one, in
     which case its old rows are requantised. Values that are not finite are stored as NaN and do not
-    enter the scale. Rows at or past ``T`` are dropped; a negative length appends nothing.
+    enter the scale. Rows at or past ``T`` are dropped; a negative length appends nothing. Nothing is
+    read on the host, so that a CUDA graph can hold the call.
     """
-    s, t = x.shape[1], cache.shape[2]
+    b, s, hkv, d = x.shape
+    t = cache.shape[2]
+    if x.numel() == 0 or t == 0:
+        return
+    n = (s + 2 * CACHE_BLOCK - 2) // CACHE_BLOCK  # blocks that s rows can touch
+    start = lengths.to(device=x.device, dtype=torch.long)[:, None]
+    inside = (start >= 0) & (start < t)
+    first = torch.where(inside, start, 0) // CACHE_BLOCK
+    at = torch.arange(b, device=x.device)[:, None]
+    row = first * CACHE_BLOCK + torch.arange(n * CACHE_BLOCK, device=x.device)  # [B, n * 32]: the window's cache rows
+    token = row - start
+    new = inside & (token >= 0) & (token < s) & (row < t)
+    touched = new.view(b, n, CACHE_BLOCK).any(-1)[:, None]  # [B, 1, n] blocks
+    old = inside & (token < 0)
+
+    rows = x[at, token.clamp(0, s - 1)].transpose(1, 2).float()  # [B, Hkv, n * 32, D]
+    size = torch.where(rows.isfinite() & new[:, None, :, None], rows.abs(), 0.0).view(b, hkv, n, CACHE_BLOCK, d).amax((3, 4))
+    block = first + torch.arange(n, device=x.device)
+    block = block.clamp(max=scale.shape[2] - 1)
+    held = scale[at, :, block].transpose(1, 2)  # [B, Hkv, n]
+    keeps = old.view(b, n, CACHE_BLOCK).any(-1)[:, None]
+    now = cache_scale(size)
+    now = torch.where(touched, torch.where(keeps, torch.maximum(now, held), now), held)
+
+    # Rows past the end stand for the last row, blocks for the last block: they write what those write.
+    row = row.clamp(max=t - 1)
     bits = cache.view(torch.uint8)
-    for b, start in enumerate(lengths.tolist()):
-        end = min(start + s, t)
-        for lo in range(start, end) if start >= 0 else ():
-            if lo != start and lo % CACHE_BLOCK:
-                continue  # the first row of each block that the rows [start, end) touch
-            block = lo // CACHE_BLOCK
-            first, hi = block * CACHE_BLOCK, min((block + 1) * CACHE_BLOCK, end)
-            rows = x[b, lo - start : hi - start].transpose(0, 1).float()  # [Hkv, rows, D]
-            size = torch.where(rows.isfinite(), rows.abs(), torch.zeros_like(rows)).amax((1, 2))
-            now = cache_scale(size)
-            if lo > first:
-                now = torch.maximum(now, scale[b, :, block])
-                held = cache[b, :, first:lo].float() * (scale[b, :, block] / now)[:, None, None]
-                bits[b, :, first:lo] = _to_e4m3(held).view(torch.uint8)
-            bits[b, :, lo:hi] = _to_e4m3(rows / now[:, None, None]).view(torch.uint8)
-            scale[b, :, block] = now
+    before = bits[at, :, row].transpose(1, 2).contiguous()
+    ratio, per_row = (f.repeat_interleave(CACHE_BLOCK, dim=2)[..., None] for f in (held / now, now))
+    value = torch.where(new[:, None, :, None], rows / per_row, before.view(cache.dtype).float() * ratio)
+    changed = (new | old) & touched[:, 0].repeat_interleave(CACHE_BLOCK, dim=1)
+    after = torch.where(changed[:, None, :, None], _to_e4m3(value).view(torch.uint8), before)
+    bits[at, :, row] = after[at, :, row - first * CACHE_BLOCK]
+    scale[at, :, block] = now[at, :, block - first]
 
 
 def rotary_append(
@@ -211,8 +228,8 @@ def cache_attention(
     p = torch.where(ok.any(-1)[:, None, None, :, None], z.softmax(dim=-1), torch.zeros_like(z))
     bad = v.isnan()
     o = torch.einsum("bkgst,bktd->bskgd", p, v.masked_fill(bad, 0.0))
-    if bool(bad.any()):  # a NaN reaches the queries that see its row, and no others
-        o = o.masked_fill(torch.einsum("bst,bktd->bskd", ok.float(), bad.float())[:, :, :, None] > 0, float("nan"))
+    # a NaN reaches the queries that see its row, and no others
+    o = o.masked_fill(torch.einsum("bst,bktd->bskd", ok.float(), bad.float())[:, :, :, None] > 0, float("nan"))
     return o.reshape(b, s, h, d).to(q.dtype)
 
 

@@ -181,3 +181,42 @@ def test_queries_of_any_finite_size(s: int, size: int) -> None:
     # so exponents are off by 2**-14, numerator and sum by 2**-14 of themselves; the roundings to bf16 may then be neighbours.
     size_v = (v.float().abs().amax((-1, -2)) * vs.amax(-1)).max()
     assert ((out.float() - base.float()).abs() <= base.float().abs() * 2.0**-7 + 2.0**-13 * size_v).all()
+
+
+@pytest.mark.parametrize("head_dim,dtype", [(32, torch.bfloat16), (32, torch.float32), (64, torch.float32), (128, torch.float16)])
+def test_decoder_with_an_8_bit_cache_captures_models_that_no_kernel_covers(head_dim: int, dtype: torch.dtype) -> None:
+    from priml_b200.inference import Decoder
+    from priml_b200.models.presets import dense_lm
+
+    torch.manual_seed(0)
+    cfg = dense_lm(vocab=512, d_model=128, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=head_dim, ffn_hidden=256,
+                   rope_theta=1e4, norm_eps=1e-6, init_std=None)  # fmt: skip
+    model = cfg.make().cuda().to(dtype).eval()
+    prompt = torch.randint(0, 512, (3, 33), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    kw = dict(batch=3, max_seq=96, kv_dtype=torch.float8_e4m3fn)
+    graphed, eager = Decoder(model, **kw), Decoder(model, **kw, cuda_graph=False)
+    kw = dict(max_new_tokens=40, temperature=0)
+    assert torch.equal(graphed.generate(prompt, **kw), eager.generate(prompt, **kw))
+    for a, c in zip(graphed.caches, eager.caches, strict=True):
+        assert torch.equal(a.k.view(torch.uint8)[:, :, :72], c.k.view(torch.uint8)[:, :, :72])
+        assert torch.equal(a.v_scale[:, :, :2], c.v_scale[:, :, :2])
+    assert len(graphed._graphs) == 1
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 32), (torch.float32, 64)])
+def test_the_torch_form_gives_the_same_bytes_on_both_devices(dtype: torch.dtype, d: int) -> None:
+    from priml_b200 import ops
+
+    b, s, hkv, t = 3, 40, 2, 100
+    g = torch.Generator().manual_seed(61)
+    x = (torch.randn(2, b, s, hkv, d, generator=g) * torch.exp2(torch.randint(-60, 61, (b, s, 1, 1), generator=g).float())).to(dtype)
+    x[0, 0, 3, 1, 2], x[1, 2, 39, 0, 0] = float("nan"), float("inf")
+    n = torch.tensor([0, 31, 70], dtype=torch.int32)
+    held = []
+    for device in ("cpu", "cuda"):
+        k, ks = filled_cache(b, hkv, t, d, seed=62, device=device)
+        v, vs = filled_cache(b, hkv, t, d, seed=63, device=device)
+        ops.rotary_append(x[0].to(device), *x.to(device), k, v, ks, vs, n.to(device))
+        held.append([z.cpu() for z in (k.float(), v.float(), ks, vs)])
+    for a, c in zip(*held, strict=True):
+        assert torch.equal(a.nan_to_num(1e9), c.nan_to_num(1e9))
