@@ -249,6 +249,21 @@ def _check_cache(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v
         raise ValueError("the caches, their scales and the lengths must be on the queries' device.")
 
 
+def _overlap(*tensors: Tensor) -> bool:
+    """Whether two (sequence, head) planes of these tensors of one shape share memory; rows within a plane are packed."""
+    x = tensors[0]
+    if not x.numel():
+        return False
+    size, plane = x.element_size(), x[0, 0].numel() * x.element_size()
+    starts = sorted(
+        t.data_ptr() + size * (i * t.stride(0) + j * t.stride(1))
+        for t in tensors
+        for i in range(t.shape[0])
+        for j in range(t.shape[1])
+    )
+    return any(b - a < plane for a, b in zip(starts, starts[1:], strict=False))
+
+
 def rotary_append(
     q: Tensor,
     k: Tensor,
@@ -290,7 +305,9 @@ def rotary_append(
     if cos is not None and (cos.ndim != 2 or cos.shape != sin.shape or not 2 <= 2 * cos.shape[1] <= q.shape[-1] or cos.shape[0] < 1):
         raise ValueError(f"cos and sin must be [positions, R/2] tables with 2 <= R <= {q.shape[-1]}, got {tuple(cos.shape)}.")
     _check_cache(q, k_cache, v_cache, k_scale, v_scale, lengths)
-    if k_cache.numel() and (k_cache.data_ptr() == v_cache.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr()):
+    if _overlap(k_cache) or _overlap(v_cache) or _overlap(k_scale) or _overlap(v_scale):
+        raise ValueError("caches and scales must not overlap themselves.")
+    if _overlap(k_cache, v_cache) or _overlap(k_scale, v_scale):
         raise ValueError("keys and values need caches and scales of their own.")
     if any(x.requires_grad for x in (q, k, v)) and torch.is_grad_enabled():
         raise RuntimeError("rotary_append has no gradient: call it under torch.no_grad().")

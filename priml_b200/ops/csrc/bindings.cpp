@@ -829,6 +829,43 @@ void check_planes(const Tensor& t, const char* name) {
            std::string(name) + " must not overlap itself");
 }
 
+// Whether two tensors of one shape, each free of overlap in itself (check_planes), share memory.
+bool share_memory(const Tensor& x, const Tensor& y) {
+  if (x.numel() == 0) return false;
+  const int64_t item = x.element_size(), plane = item * (x.dim() == 4 ? x.size(2) * x.size(3) : x.size(2));
+  const int64_t n[2] = {x.size(0), x.size(1)};
+  auto start = [&](const Tensor& t) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data_ptr())); };
+  auto span = [&](const Tensor& t) {
+    return plane + item * ((n[0] - 1) * t.stride(0) + (n[1] - 1) * t.stride(1));  // bytes from first to last
+  };
+  const int64_t x0 = start(x), y0 = start(y);
+  if (x0 + span(x) <= y0 || y0 + span(y) <= x0) return false;
+  if ((n[0] <= 1 || x.stride(0) == y.stride(0)) && (n[1] <= 1 || x.stride(1) == y.stride(1))) {
+    // Planes meet if |y0 - x0 + i outer + j inner| < plane for steps i, j within the counts. The inner planes of
+    // one outer step span no more than `outer`, and a plane no more than `inner`: the steps on either side of the
+    // root are the only candidates.
+    const int o = n[0] <= 1 ? 1 : (n[1] <= 1 ? 0 : (x.stride(0) >= x.stride(1) ? 0 : 1));
+    auto around = [](int64_t distance, int64_t stride, int64_t count, auto&& hits) {
+      if (count <= 1) return hits(distance);
+      const int64_t low = -(distance >= 0 ? (distance + stride - 1) / stride : distance / stride);  // floor(-distance / stride)
+      for (const int64_t i : {low, low + 1})
+        if (i > -count && i < count && hits(distance + i * stride)) return true;
+      return false;
+    };
+    return around(y0 - x0, item * x.stride(o), n[o], [&](int64_t d) {
+      return around(d, item * x.stride(1 - o), n[1 - o], [&](int64_t e) { return e < plane && -e < plane; });
+    });
+  }
+  std::vector<int64_t> starts;
+  for (const Tensor* t : {&x, &y})
+    for (int64_t b = 0; b < n[0]; ++b)
+      for (int64_t h = 0; h < n[1]; ++h) starts.push_back(start(*t) + item * (b * t->stride(0) + h * t->stride(1)));
+  std::sort(starts.begin(), starts.end());
+  for (size_t i = 1; i < starts.size(); ++i)
+    if (starts[i] - starts[i - 1] < plane) return true;
+  return false;
+}
+
 // Channels contiguous and rows 16-byte aligned, as the vector loads need them.
 Tensor rows16(const Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
@@ -856,12 +893,12 @@ Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, Tenso
   check_cache(k_cache, k_scale, q_, B, Hkv, T, D, "k");
   check_cache(v_cache, v_scale, q_, B, Hkv, T, D, "v");
   const Tensor lengths = lengths_of(lengths_, q_, B);
-  PB_VALUE(k_cache.numel() == 0 || (k_cache.data_ptr() != v_cache.data_ptr() && k_scale.data_ptr() != v_scale.data_ptr()),
-           "keys and values need caches and scales of their own");
   check_planes(k_cache, "k cache");
   check_planes(v_cache, "v cache");
   check_planes(k_scale, "k scales");
   check_planes(v_scale, "v scales");
+  PB_VALUE(!share_memory(k_cache, v_cache) && !share_memory(k_scale, v_scale),
+           "keys and values need caches and scales of their own");
   PB_VALUE(cos.has_value() == sin.has_value(), "cos and sin come together");
   PB_VALUE(T < (1LL << 31) - 64 && B * s < (1LL << 30) && B * Hkv * (s / pb::kCacheBlock + 2) < (1LL << 29),
            "sizes out of range");

@@ -2,9 +2,11 @@
 
 from __future__ import annotations
 
+import pytest
 import torch
 from torch._subclasses import FakeTensorMode
 
+from priml_b200 import ops
 from priml_b200.ops import reference
 
 
@@ -20,3 +22,36 @@ def test_the_torch_form_reads_nothing_on_the_host() -> None:
         out = reference.rotary_append(q, x, x, k, v, ks, vs, n, table, table, False)
         seen = reference.cache_attention(out, k, v, ks, vs, n, scale=0.25, window=7, offset=s)
     assert seen.shape == (b, s, h, d)
+
+
+def _halves() -> tuple[list, list]:
+    """(k, v, k scales, v scales) cut from one buffer each: ones that share a part, ones that do not."""
+    rows = torch.zeros(2, 4, 64, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    scales, own = torch.ones(2, 4, 2), torch.ones(2, 2, 2)
+    pairs = rows.view(4, 2, 64, 64)
+    shared = [
+        (rows[:, :2], rows[:, 1:3], scales[:, :2], scales[:, 2:]),  # a head of both
+        (rows[:, 0:4:2], rows[:, 2:4], scales[:, :2], scales[:, 2:]),  # strides of their own
+        (rows[:, :2], rows[:, 2:], scales[:, 1:3], scales[:, 2:]),
+        (rows[:, :2], rows.flatten()[64 * 64 + 1024 :][: 4 * 64 * 64].view(2, 2, 64, 64), own, own.clone()),  # half a head
+        (rows[:, :2], rows[:, :2], own, own.clone()),
+        (rows[:1, :2].expand(2, -1, -1, -1), rows[:, 2:], own, own.clone()),  # one cache for both sequences
+    ]
+    apart = [
+        (rows[:, :2], rows[:, 2:], scales[:, :2], scales[:, 2:]),
+        (rows[:, 0::2], rows[:, 1::2], scales[:, 0::2], scales[:, 1::2]),
+        (rows[:, :2], rows[:, 2:].clone(), scales[:, 2:], scales[:, :2].clone()),
+        (pairs[:2], pairs[2:], own, own.clone()),
+        (pairs[0::2], pairs[1::2], scales.view(4, 2, 2)[0::2], scales.view(4, 2, 2)[1::2]),
+        (pairs.transpose(0, 1)[:, :2], pairs.transpose(0, 1)[:, 2:], own, own.clone()),  # heads outside sequences
+    ]
+    return shared, apart
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_append_refuses_caches_that_share_a_part(which: int) -> None:
+    shared, apart = _halves()
+    q, x, n = torch.zeros(2, 1, 4, 64), torch.zeros(2, 1, 2, 64), torch.tensor([3, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="of their own|overlap"):
+        ops.rotary_append(q, x, x, *shared[which], n)
+    assert ops.rotary_append(q, x, x, *apart[which], n) is q

@@ -220,3 +220,22 @@ def test_the_torch_form_gives_the_same_bytes_on_both_devices(dtype: torch.dtype,
         held.append([z.cpu() for z in (k.float(), v.float(), ks, vs)])
     for a, c in zip(*held, strict=True):
         assert torch.equal(a.nan_to_num(1e9), c.nan_to_num(1e9))
+
+
+def test_append_refuses_caches_that_share_a_part() -> None:
+    """(Refused before anything is launched.)"""
+    from priml_b200 import ops
+
+    q = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    n = _ints([3, 4])
+    from tests.test_cache8_edges_cpu import _halves
+
+    with torch.device("cuda"):
+        shared, apart = _halves()
+    for case in shared:
+        with pytest.raises(ValueError, match="of their own|overlap"):
+            ops.rotary_append(q, x, x, *case, n)
+    for case in apart:
+        assert ops.rotary_append(q, x, x, *case, n) is q
+    _status_clean()
