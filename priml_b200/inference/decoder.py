@@ -90,11 +90,16 @@ class Decoder:
                                    device=self.device, dtype=self.dtype)  # fmt: skip
 
     def _fp8_cache(self, attn: Any) -> Fp8KVCache:
-        cos = sin = None
-        if type(attn.rope) is RoPE:  # factors of other embeddings are the module's to apply
-            cos, sin = (f[:, 0].float().contiguous() for f in attn.rope.table(self.max_seq, self.device))
+        cos, sin = self._rotary_tables(attn.rope)
         return Fp8KVCache.alloc(self.state, heads=attn.num_heads_kv, channels_head=attn.channels_head,
                                 device=self.device, cos=cos, sin=sin)  # fmt: skip
+
+    def _rotary_tables(self, rope: Any) -> tuple[Tensor | None, Tensor | None]:
+        """Factors of ``max_seq`` positions, made apart from the table that the module keeps for its own calls."""
+        if type(rope) is not RoPE:  # factors of other embeddings are the module's to apply
+            return None, None
+        cos, sin = (f[:, 0].float().contiguous() for f in rope(torch.arange(self.max_seq, device=self.device)))
+        return cos, sin
 
     # ------------------------------------------------------------------ state
     def reset(self, rows: slice | None = None) -> None:

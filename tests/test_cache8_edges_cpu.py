@@ -55,3 +55,17 @@ def test_append_refuses_caches_that_share_a_part(which: int) -> None:
     with pytest.raises(ValueError, match="of their own|overlap"):
         ops.rotary_append(q, x, x, *shared[which], n)
     assert ops.rotary_append(q, x, x, *apart[which], n) is q
+
+
+def test_a_decoder_leaves_the_model_its_rotary_table() -> None:
+    """A captured training step reads the table's memory, and the next one would have to make it again."""
+    from priml_b200.inference import Decoder
+    from priml_b200.models.presets import tiny_lm
+
+    model = tiny_lm().make().eval()
+    rope = model.blocks[0].attn.rope
+    table = rope.table(24, torch.device("cpu"))
+    dec = Decoder(model, batch=1, max_seq=64, kv_dtype=torch.float8_e4m3fn)
+    assert rope.table(24, torch.device("cpu"))[0] is table[0]
+    for own, whole in zip((dec.caches[0].cos, dec.caches[0].sin), rope(torch.arange(64)), strict=True):
+        assert torch.equal(own, whole[:, 0])
