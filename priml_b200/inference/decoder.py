@@ -76,7 +76,9 @@ class Decoder:
         if kv_dtype not in (None, self.dtype, torch.float8_e4m3fn):
             raise ValueError(f"kv_dtype must be {self.dtype} or torch.float8_e4m3fn, got {kv_dtype}.")
         make = self._fp8_cache if kv_dtype == torch.float8_e4m3fn else self._static_cache
-        self.caches: list[StaticKVCache | Fp8KVCache] = [make(b.attn) for b in blocks]
+        self.caches: list[StaticKVCache | Fp8KVCache] = []
+        for b in blocks:
+            self.caches.append(make(b.attn))
         self.host_lengths = [0] * batch
         self.use_graph = cuda_graph and self.device.type == "cuda"
         self._tok = torch.zeros(batch, dtype=torch.long, device=self.device)
@@ -95,10 +97,14 @@ class Decoder:
                                 device=self.device, cos=cos, sin=sin)  # fmt: skip
 
     def _rotary_tables(self, rope: Any) -> tuple[Tensor | None, Tensor | None]:
-        """Factors of ``max_seq`` positions, made apart from the table that the module keeps for its own calls."""
+        """Factors of ``max_seq`` positions, made apart from the table that the module keeps for its own calls; layers
+        with equal factors share them."""
         if type(rope) is not RoPE:  # factors of other embeddings are the module's to apply
             return None, None
         cos, sin = (f[:, 0].float().contiguous() for f in rope(torch.arange(self.max_seq, device=self.device)))
+        for held in self.caches:
+            if held.cos is not None and torch.equal(held.cos, cos) and torch.equal(held.sin, sin):
+                return held.cos, held.sin
         return cos, sin
 
     # ------------------------------------------------------------------ state

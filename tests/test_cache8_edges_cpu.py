@@ -69,3 +69,18 @@ def test_a_decoder_leaves_the_model_its_rotary_table() -> None:
     assert rope.table(24, torch.device("cpu"))[0] is table[0]
     for own, whole in zip((dec.caches[0].cos, dec.caches[0].sin), rope(torch.arange(64)), strict=True):
         assert torch.equal(own, whole[:, 0])
+
+
+def test_layers_with_equal_factors_share_one_rotary_table() -> None:
+    from priml_b200.inference import Decoder
+    from priml_b200.models.presets import tiny_lm
+    from priml_b200.models.rope import RoPE
+
+    model = tiny_lm().make().eval()
+    dec = Decoder(model, batch=1, max_seq=64, kv_dtype=torch.float8_e4m3fn)
+    a, c = dec.caches
+    assert a.cos is c.cos and a.sin is c.sin
+    model.blocks[1].attn.rope = RoPE.Config(32, base=5e5).make()
+    other = Decoder(model, batch=1, max_seq=64, kv_dtype=torch.float8_e4m3fn)
+    a, c = other.caches
+    assert torch.equal(a.cos, dec.caches[0].cos) and not torch.equal(a.cos, c.cos)
