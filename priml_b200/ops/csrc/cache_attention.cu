@@ -673,14 +673,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) cache_attn_merge_kernel(cons
 
 template <int D, int RT>
 int ctas_per_sm() {
-  static int cached = 0;
-  if (cached == 0) {
+  static const int n = [] {  // (threads that come here first together wait for one of them)
     cudaFuncSetAttribute(cache_attn_kernel<D, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, RT>::kBytes);
-    int n = 0;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_attn_kernel<D, RT>, kWarps * 32, Cfg<D, RT>::kBytes);
-    cached = n < 1 ? 1 : n;
-  }
-  return cached;
+    int found = 0;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&found, cache_attn_kernel<D, RT>, kWarps * 32, Cfg<D, RT>::kBytes);
+    return found < 1 ? 1 : found;
+  }();
+  return n;
 }
 
 template <int D, int RT>

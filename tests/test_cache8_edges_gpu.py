@@ -239,3 +239,37 @@ def test_append_refuses_caches_that_share_a_part() -> None:
     for case in apart:
         assert ops.rotary_append(q, x, x, *case, n) is q
     _status_clean()
+
+
+def test_threads_that_call_first_together() -> None:
+    """Several host threads, each on its own stream, in a process that has not called the operator before."""
+    import subprocess
+    import sys
+
+    code = """
+import threading
+import torch
+from priml_b200 import ops
+from tests.cache8_cases import filled_cache
+
+k, ks = filled_cache(2, 2, 500, 64, seed=1, device="cuda")
+v, vs = filled_cache(2, 2, 500, 64, seed=2, device="cuda")
+n = torch.tensor([500, 130], dtype=torch.int32, device="cuda")
+q = torch.randn(2, 1, 8, 64, device="cuda").bfloat16()
+torch.cuda.synchronize()
+outs = [None] * 6
+gate = threading.Barrier(6)
+
+def run(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        gate.wait()
+        outs[i] = ops.cache_attention(q, k, v, ks, vs, n)
+        torch.cuda.current_stream().synchronize()
+
+threads = [threading.Thread(target=run, args=(i,)) for i in range(6)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert all(torch.equal(o, outs[0]) for o in outs) and outs[0].isfinite().all()
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
