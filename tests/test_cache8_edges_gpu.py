@@ -241,6 +241,69 @@ def test_append_refuses_caches_that_share_a_part() -> None:
     _status_clean()
 
 
+def _telling_cache(b: int, hkv: int, t: int, d: int, seed: int) -> tuple[Tensor, Tensor]:
+    """Values that are positive in one channel per block of 32 rows, ``block % d``, and zero elsewhere: an output channel
+    is the sum of few blocks' parts, none of which can be lost unseen."""
+    g = torch.Generator().manual_seed(seed)
+    nb = -(-t // BLOCK)
+    x = torch.zeros(b, hkv, nb, BLOCK, d)
+    x[:, :, torch.arange(nb), :, torch.arange(nb) % d] = 1 + torch.rand(nb, b, hkv, BLOCK, generator=g)
+    x *= torch.exp2(torch.randint(-1, 2, (b, hkv, nb, 1, 1), generator=g).float())
+    scale = torch.exp2(torch.ceil(torch.log2(x.amax((-1, -2)) / 448)))
+    rows = (x / scale[..., None, None]).to(torch.float8_e4m3fn).view(b, hkv, nb * BLOCK, d)
+    return rows[:, :, :t].contiguous().cuda(), scale.cuda()
+
+
+LONG = [  # B, s, H, Hkv, T, D, ends, window
+    (1, 1, 8, 8, 9000, 64, [9000], None),
+    (16, 1, 8, 8, 2100, 64, [2100] * 16, None),
+    (4, 2, 32, 4, 12000, 128, [12000, 11999, 11990, 2], None),
+    (1, 1, 16, 1, 60001, 128, [60001], None),  # one item over the whole grid
+    (3, 5, 8, 1, 9001, 64, [9001, 5000, 33], None),  # many-row form, both groups on the same rows
+    (1, 520, 2, 1, 3001, 128, [2999], None),
+    (1, 150, 4, 2, 20000, 128, [19999], None),
+    (2, 260, 2, 2, 6000, 64, [6000, 5500], 3000),
+    (1, 2100, 2, 1, 2100, 128, [2100], None),  # a whole fresh prompt
+    (2, 1300, 4, 2, 1300, 64, [1300, 1300], 100),
+]
+
+
+@pytest.mark.parametrize("b,s,h,hkv,t,d,ends,window", LONG)
+def test_every_block_of_a_long_run_is_in_the_output(b, s, h, hkv, t, d, ends, window) -> None:  # noqa: ANN001
+    from priml_b200 import ops
+
+    k, ks = filled_cache(b, hkv, t, d, seed=51, device="cuda")
+    v, vs = _telling_cache(b, hkv, t, d, seed=52)
+    q = _queries(b, s, h, d, seed=53) * 0.25
+    n = _ints(ends)
+    out = ops.cache_attention(q, k, v, ks, vs, n, window=window)
+    again = ops.cache_attention(q, k, v, ks, vs, n, window=window)
+    _status_clean()
+    assert torch.equal(out, again)  # sums in a fixed order
+    want = attend64(q, k, v, ks, vs, ends, window=window)
+    limit = _limit(want, want)  # V >= 0
+    assert ((out.cpu().double() - want).abs() <= limit).all()
+    # The same result without one block of keys is out of that limit, for every block of which a query sees half. (One
+    # key of the 15 x 32 that share a channel in the longest case is 2**-9 of it, the limit 2**-8 + 2**-11 + 2**-13.)
+    block = torch.arange(t) // BLOCK
+    for i in range(b):
+        for head in (0, h - 1):
+            kv = head // (h // hkv)
+            pos = ends[i] - 1
+            lo = 0 if window is None else max(0, pos - window)
+            kk = k[i, kv].cpu().double() * ks[i, kv].cpu().double()[block, None]
+            vv = v[i, kv].cpu().double() * vs[i, kv].cpu().double()[block, None]
+            p = (kk[lo : pos + 1] @ q[i, s - 1, head].cpu().double() * d**-0.5).softmax(-1)
+            full = p @ vv[lo : pos + 1]
+            torch.testing.assert_close(full, want[i, s - 1, head])
+            seen = block[lo : pos + 1]
+            blocks, rows = seen.unique(return_counts=True)
+            for j in blocks[rows >= BLOCK // 2].tolist() if len(blocks) > 1 else []:
+                keep = seen != j
+                lost = p[keep] @ vv[lo : pos + 1][keep] / p[keep].sum()
+                assert ((lost - full).abs() > 2 * limit[i, s - 1, head]).any(), (i, head, j)
+
+
 def test_threads_that_call_first_together() -> None:
     """Several host threads, each on its own stream, in a process that has not called the operator before."""
     import subprocess
