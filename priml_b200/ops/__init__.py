@@ -107,7 +107,7 @@ def rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, interleave: bool =
     The pairs are channels ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleave``. The rotation is
     computed in fp32 and rounded once. On CUDA q and k take one kernel (bf16, fp16, fp32), and its
     transpose in the backward; odd head widths and factors that need a gradient take the torch operations,
-    and so do calls under ``torch.func`` transforms, forward-mode AD, ``torch.compile`` and fake tensors.
+    and so do calls under ``torch.func`` transforms, forward-mode AD, ``torch.compile``, tracing and fake tensors.
     """
     if use_native(q):
         from priml_b200.ops import functional

@@ -78,3 +78,21 @@ def test_compiled_without_a_graph_break() -> None:
     run = torch.compile(lambda *a: RoPE.rotate(*a, True), fullgraph=True, backend="eager")
     for a, c in zip(run(q, k, cos, sin), RoPE.rotate(q, k, cos, sin, True), strict=True):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("interleave", [False, True])
+def test_traced_graphs_rotate_the_inputs_that_they_are_given(interleave: bool) -> None:
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from priml_b200.models.rope import RoPE
+
+    q, k, cos, sin = _inputs()
+
+    def turn(a: torch.Tensor, c: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return RoPE.rotate(a, c, cos, sin, interleave)
+
+    for run in (make_fx(turn)(q, k), torch.jit.trace(turn, (q, k))):
+        for a, c in zip(run(q + 1, k * 2), turn(q + 1, k * 2), strict=True):
+            # A traced graph may be compiled, with a product and a sum rounded once together: the unrounded product, under
+            # 2**3, is then off by at most 2**-22. A result held from the tracing is off by one and more.
+            torch.testing.assert_close(a, c, rtol=0, atol=2.0**-21)
