@@ -62,7 +62,8 @@ class Decoder:
         cuda_graph: bool = True,
     ) -> None:
         """``kv_dtype=torch.float8_e4m3fn`` keeps keys and values in 8 bits (:class:`Fp8KVCache`); by default
-        they have the activations' ``dtype``."""
+        they have the activations' ``dtype``. Its kernels cover bf16 models with heads of 64 or 128; others
+        take torch operations, in the same captured step."""
         from priml_b200.models.attention import SelfAttention
 
         blocks = list(getattr(model, "blocks", []))

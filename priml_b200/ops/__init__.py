@@ -292,7 +292,8 @@ def rotary_append(
     not finite are stored as NaN. Tokens past ``T`` are not stored. Returns the rotated q, or ``q`` itself
     where nothing is rotated.
 
-    On CUDA with bf16 and 64 or 128 channels a head this is one kernel (``csrc/rotary.cu``).
+    On CUDA with bf16 and 64 or 128 channels a head this is one kernel (``csrc/rotary.cu``); others take torch
+    operations on the device.
     """
     if use_native(q) and q.dtype == k.dtype == v.dtype == torch.bfloat16 and q.shape[-1] in (64, 128):
         return native().rotary_append(q, k, v, k_cache, v_cache, k_scale, v_scale, lengths, cos, sin, interleave)
@@ -328,14 +329,16 @@ def cache_attention(
 ) -> Tensor:
     """Attention of each sequence's last tokens over its 8-bit cache (see :func:`rotary_append`).
 
-    ``q`` is ``[B, H, D]`` (one token per sequence) or ``[B, s, H, D]`` (a chunk). ``lengths[b] + offset``
-    rows of sequence ``b`` are filled, the chunk's own included: query ``i`` stands at position
-    ``lengths[b] + offset - s + i`` and sees the rows up to its own, with ``window`` only those not more
-    than ``window`` behind it. A query that sees no row gives zeros; rows that a query does not see may
-    hold anything. Query head ``h`` reads KV head ``h // (H / Hkv)``. The lengths stay on the device, so
+    ``q`` is ``[B, H, D]`` (one token per sequence) or ``[B, s, H, D]`` (a chunk). ``n = min(lengths[b] + offset, T)``
+    rows of sequence ``b`` are filled, the chunk's own included: query ``i`` stands at position ``n - s + i``
+    (so a chunk that ran past the cache's end stands at the last ``s`` rows) and sees the rows up to its own,
+    with ``window`` only those not more than ``window`` behind it. A query that sees no row gives zeros; rows that a query does not see may
+    hold anything; a NaN among the values reaches its own channel of the queries that see its row. Query head ``h`` reads KV head ``h // (H / Hkv)``. The lengths stay on the device, so
     the call can be captured in a CUDA graph. Returns ``q``'s shape.
 
-    On CUDA with bf16 queries and 64 or 128 channels a head this runs ``csrc/cache_attention*.cu``.
+    On CUDA with bf16 queries and 64 or 128 channels a head this runs ``csrc/cache_attention*.cu``; others take
+    torch operations on the device. The kernels round the weights to f16 (half a step is 2**-11 of one) and keep a
+    query's channels exactly down to 2**-30 of the largest one.
     """
     if window is not None and window < 0:
         window = None

@@ -15,10 +15,11 @@
 // the memory and the products.
 //
 // Measured (B200, 32 query and 8 KV heads): 64 sequences of 8192 tokens, heads of 128, 1.08 GB, in 175 us,
-// 6.15 TB/s (a plain copy: 6.5), while the SMs run at 1965 MHz, and 193 us once the power cap has them at 1700;
+// 6.15 TB/s (a plain copy: 6.5), while the SMs run at 1965 MHz, and 197 us once the power cap has them at 1700;
 // one sequence of 1000 tokens, heads of 64, 14 us, of which the kernels take 8. What is left is the latency of
 // a 32-key step that three CTAs per SM do not quite hide. Other forms: the bytes loaded straight into
-// registers 196 us and, at 16 rows, 41 us where this took 38.6 (nine sequences of 1 to 100001 tokens); a
+// registers 196 us where this took 193 and, at 16 rows, 41 us where this took 38.6 (nine sequences of 1 to 100001
+// tokens; 36.6 us now, with the merge launched early); a
 // ring whose lanes copy only what they read themselves (half lines of K) 240 us when direct loads took 214;
 // four CTAs per SM 226 us (registers spill); a second wave of short runs for the SMs that finish first (equal
 // runs end 25 % apart) 208 us, its CTAs' starts costing more than they even out.
@@ -36,7 +37,7 @@
 // w = 2^(s + ev - m), m the running maximum of s + ev, while the row sum adds w 2^-ev. So the weights
 // fit f16 whatever the scales. Query rows are normalised by a power of two to fit f16 (exact down to 2^-30
 // of the row's largest channel, see row_power; the factor goes to the scores). Weights are rounded to f16 as 2^10 w: half a step is 2^-11 relative down
-// to w = 2^-24, less than bf16's 2^-9 of the output, and far tails stay above zero.
+// to w = 2^-24, less than the 2^-8 that half a step of bf16 is of the output, and far tails stay above zero.
 //
 // Work split: the key blocks of all (sequence, KV head, row group) items form one list, cut into
 // equal runs over the grid on the device from the lengths, so ragged batches load all SMs alike

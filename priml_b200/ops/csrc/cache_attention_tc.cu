@@ -27,7 +27,7 @@
 // next piece while the softmax warps finish the last.
 //
 // Measured (B200, D = 128): a 2048-token prompt chunk that ends a cache of 32768, 32 + 8 heads, 1.07 TFLOP in
-// 1.23 ms (863 TFLOP/s under the power cap). The tensor cores wait for the softmax warps'
+// 1.22 to 1.24 ms (860 to 872 TFLOP/s under the power cap). The tensor cores wait for the softmax warps'
 // chain per 64 keys (score load, exponent, weight store), whose latency two buffers per group hide in part.
 // Sixteen softmax warps of 64 registers were slower (1.70 against 1.29 ms: the rows' state spills), as was raw
 // e4m3 staged through shared memory by bulk copies. Five tokens each of 8 sequences take 69 us, bound by the

@@ -18,6 +18,9 @@
 //
 // Both are bound by their bytes: each value is read and written once. Measured (B200, bf16):
 //   rotation  8 x 2048 tokens, 32 + 8 heads of 128, 32 turned: 335 MB in 58 us, 5.8 TB/s (a plain copy: 6.5)
+//             34 turned (a multiple of 2 alone: one channel per load) 168 us, 36 (two per load) 117 us: bound by the
+//             requests in flight, each moving 2 or 4 bytes. The presets turn 32, 64 or 128 channels, so these widths
+//             have no form of their own (the torch operations take 885 us).
 //   append    4 x 2048 tokens, 32 + 8 heads of 128: 186 MB in 53 us, 3.5 TB/s; one token for 64 sequences 9 us,
 //             which is the host's time for the call
 #include <cuda_bf16.h>
