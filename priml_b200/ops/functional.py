@@ -16,7 +16,6 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 from torch.autograd import forward_ad
-from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from priml_b200.ops._loader import native
 
@@ -411,10 +410,15 @@ class _Rotary(torch.autograd.Function):
 
 def traced(*tensors: Tensor) -> bool:
     """Whether a compiled autograd node must not see these tensors: something else than their data is wanted of them."""
+    if torch.compiler.is_compiling():
+        return True
+    if torch._C._len_torch_dispatch_stack() > 0:
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            return True
     return (
-        torch.compiler.is_compiling()
-        or torch.jit.is_tracing()
-        or (torch._C._len_torch_dispatch_stack() > 0 and get_proxy_mode() is not None)
+        torch.jit.is_tracing()
         or torch._C._are_functorch_transforms_active()
         or any(type(t) not in (Tensor, torch.nn.Parameter) for t in tensors)
         or (forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
