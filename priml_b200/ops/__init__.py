@@ -255,6 +255,9 @@ def _overlap(*tensors: Tensor) -> bool:
     if not x.numel():
         return False
     size, plane = x.element_size(), x[0, 0].numel() * x.element_size()
+    if all(t.is_contiguous() for t in tensors):  # what most caches are: no need to look at every plane
+        starts = sorted(t.data_ptr() for t in tensors)
+        return any(b - a < x.numel() * size for a, b in zip(starts, starts[1:], strict=False))
     starts = sorted(
         t.data_ptr() + size * (i * t.stride(0) + j * t.stride(1))
         for t in tensors
