@@ -36,8 +36,9 @@
 // One scale belongs to one 32-key step: K's multiplies the scores; V's goes into the weights,
 // w = 2^(s + ev - m), m the running maximum of s + ev, while the row sum adds w 2^-ev. So the weights
 // fit f16 whatever the scales. Query rows are normalised by a power of two to fit f16 (exact down to 2^-30
-// of the row's largest channel, see row_power; the factor goes to the scores). Weights are rounded to f16 as 2^10 w: half a step is 2^-11 relative down
-// to w = 2^-24, less than the 2^-8 that half a step of bf16 is of the output, and far tails stay above zero.
+// of the row's largest channel, see row_power; the factor goes to the scores). Weights are rounded to f16 as
+// 2^10 w: half a step is 2^-11 relative down to w = 2^-24, less than the 2^-8 that half a step of bf16 is of the
+// output, and far tails stay above zero.
 //
 // Work split: the key blocks of all (sequence, KV head, row group) items form one list, cut into
 // equal runs over the grid on the device from the lengths, so ragged batches load all SMs alike

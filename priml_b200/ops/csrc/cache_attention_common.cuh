@@ -73,8 +73,8 @@ __device__ __forceinline__ uint32_t nan_bits(uint32_t w) {
 
 // A query row times the power of two `down` fits f16; `up` undoes it. The row's largest magnitude goes to [2^13, 2^14):
 // f16 ends at 2^16 and its least step is 2^-24, so channels down to 2^-30 of the largest keep all their bits (bf16 has
-// eight) and smaller ones are off by at most 2^-38 of the largest. Zero rows and rows with an infinity stay as they are;
-// rows under 2^-113 go as far up as `up` stays a normal number.
+// eight) and smaller ones are off by at most 2^-38 of the largest. Rows of zeros or subnormal numbers and rows with an
+// infinity stay as they are; rows under 2^-113 go as far up as `up` stays a normal number.
 __device__ __forceinline__ void row_power(float amax, float& down, float& up) {
   const uint32_t ex = (__float_as_uint(amax) >> 23) & 255u;
   const bool plain = ex == 0u || ex == 255u;
