@@ -335,9 +335,10 @@ def cache_attention(
     ``q`` is ``[B, H, D]`` (one token per sequence) or ``[B, s, H, D]`` (a chunk). ``n = min(lengths[b] + offset, T)``
     rows of sequence ``b`` are filled, the chunk's own included: query ``i`` stands at position ``n - s + i``
     (so a chunk that ran past the cache's end stands at the last ``s`` rows) and sees the rows up to its own,
-    with ``window`` only those not more than ``window`` behind it. A query that sees no row gives zeros; rows that a query does not see may
-    hold anything; a NaN among the values reaches its own channel of the queries that see its row. Query head ``h`` reads KV head ``h // (H / Hkv)``. The lengths stay on the device, so
-    the call can be captured in a CUDA graph. Returns ``q``'s shape.
+    with ``window`` only those not more than ``window`` behind it. A query that sees no row gives zeros; rows
+    that a query does not see may hold anything; a NaN among the values reaches its own channel of the queries
+    that see its row. Query head ``h`` reads KV head ``h // (H / Hkv)``. The lengths stay on the device, so the
+    call can be captured in a CUDA graph. Returns ``q``'s shape.
 
     On CUDA with bf16 queries and 64 or 128 channels a head this runs ``csrc/cache_attention*.cu``; others take
     torch operations on the device. The kernels round the weights to f16 (half a step is 2**-11 of one) and keep a
